@@ -351,6 +351,78 @@ EXL3_API int exl3_ar_add_norm_rot(const exl3_peer_group* g, int slot, const void
 /* Status bits of the group's own flag block (4 = a wait for another rank timed out). */
 EXL3_API int exl3_peer_status(const exl3_peer_group* g, uint32_t* status);
 
+/*
+ * Paged serving: a batch of sequences over a cache of fixed-size pages (no counterpart in the reference,
+ * whose cache belongs to oMLX and attention to the model library).
+ *
+ * k_pages / v_pages: (num_pages, hkv, page_size, head_dim), fp16 or bf16 (dtype), contiguous, 16-byte
+ * aligned. Sequence s feeds rows cu_rows[s] .. cu_rows[s + 1] - 1 of a call (cu_rows[0] = 0,
+ * cu_rows[seqs] = rows) and holds lens[s] positions once they are appended: its row i is at position
+ * lens[s] - (cu_rows[s + 1] - cu_rows[s]) + i. Position p lives in page page_table[s][p / page_size].
+ * A row at a negative position is padding: nothing is appended for it and its output is zero. All
+ * tables are int32 on the device and read by the kernels alone (a captured graph follows their contents).
+ * What they name outside the pool, the page table or the rotation table is left out and sets bit 8 of
+ * *status; a pipeline wait that gave up sets bit 1.
+ */
+typedef struct exl3_paged_desc {
+    void* k_pages;
+    void* v_pages;
+    const int32_t* page_table;   /* (seqs, table_cols) */
+    const int32_t* cu_rows;      /* (seqs + 1) */
+    const int32_t* lens;         /* (seqs) */
+    int32_t seqs, rows, table_cols;
+    int32_t num_pages, page_size;  /* page_size: a power of two, 16 or more */
+    int32_t hkv, head_dim;         /* head_dim 64 or 128 */
+    int32_t dtype;                 /* EXL3_F16 or EXL3_BF16 */
+} exl3_paged_desc;
+
+/*
+ * After the q/k/v projections: per-head RMSNorm of q and k (q_norm_w / k_norm_w (head_dim) in in_dtype, or
+ * null for none), rotate-half rotary embedding of the first 2 * rope_half elements (cos / sin fp32
+ * (rope_rows, rope_half); rope_half a multiple of 8, up to head_dim / 2), k and v appended to the pages at each row's position, q to
+ * q_out (rows, hq, head_dim) in the cache's dtype. Computed in fp32 and rounded once. q (rows, hq *
+ * head_dim), k and v (rows, hkv * head_dim) fp16 or bf16 with the given row strides in elements.
+ */
+EXL3_API int exl3_paged_qkv_post(const exl3_paged_desc* batch, const void* q, const void* k, const void* v,
+                                 long long q_stride, long long k_stride, long long v_stride, int in_dtype, int hq,
+                                 const void* q_norm_w, const void* k_norm_w, float eps, const float* cos_table,
+                                 const float* sin_table, int rope_rows, int rope_half, void* q_out, uint32_t* status,
+                                 void* stream);
+
+/*
+ * Attention of the batch's rows over their sequences' pages: out[r, h] = softmax_j(scale * q[r, h] . K[j, h / g])
+ * V[j, h / g] over positions j <= the row's own, g = hq / hkv. q and out (rows, hq, head_dim) in the
+ * cache's dtype, 16-byte aligned; q's rows q_stride elements apart. fp32 scores and statistics. The
+ * workspace (exl3_paged_attn_workspace bytes; its first EXL3_PAGED_HEADER_BYTES zeroed once, left zero by
+ * every completed call) must not be shared by calls that overlap.
+ */
+#define EXL3_PAGED_HEADER_BYTES 4096
+EXL3_API int exl3_paged_attn_workspace(const exl3_paged_desc* batch, int hq, size_t* bytes);
+EXL3_API int exl3_paged_attn(const exl3_paged_desc* batch, const void* q, long long q_stride, int hq, float scale,
+                             void* out, void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
+
+/*
+ * Verification of drafted tokens (speculative sampling; no counterpart in the reference, where oMLX's MTP
+ * scheduler does it). Sequence s has target rows cu_rows[s] .. cu_rows[s + 1] - 1, one or more: all but its
+ * last judge one draft each; row r of sequence s judges draft r - s (drafts packed in row order, rows - seqs
+ * of them). With p = softmax(target / T) and q = softmax(draft / T) (draft null: q is one-hot at the drafted
+ * token; T = 0: p is one-hot at the row's first largest logit and q at the drafted token):
+ *   accept_prob[i] = min(1, p(x_i) / q(x_i)); drafts are accepted while u[i] < accept_prob[i];
+ *   the next token is the first v with the largest w(v) / noise[s][v], w = max(0, p - q) at the row of the
+ *   first rejected draft (p where that is zero everywhere) or p at the row after the last accepted one.
+ * noise: positive, exponentially distributed (that makes the race a draw from w). tokens_out (seqs,
+ * max_drafts + 1): the accepted drafts, the next token, then -1; count = accepted + 1. A row whose logits
+ * are all -inf (or not numbers) accepts nothing and gives token -1. Drafts past max_drafts are not looked at.
+ * target (rows, n) and draft (rows - seqs, n) in one dtype (fp16, bf16, fp32), rows ld elements apart;
+ * temperature (seqs) may be null (1).
+ */
+EXL3_API int exl3_verify_workspace(int rows, int seqs, int n, size_t* bytes);
+EXL3_API int exl3_verify_drafts(const void* target, long long target_ld, const void* draft, long long draft_ld, int dtype,
+                                int rows, int seqs, int n, const long long* draft_tokens, const int32_t* cu_rows,
+                                const float* temperature, const float* u, const float* noise, long long noise_ld,
+                                int max_drafts, long long* tokens_out, int32_t* count, float* accept_prob,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

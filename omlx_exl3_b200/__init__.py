@@ -6,6 +6,9 @@ C ABI in include/exl3_b200.h (libexl3b200.so).
 """
 from .kernels import MAX_GEMV_ROWS, TrellisGemvPlan, decode_wt, had_svh, norm_rot, rot, swiglu_rot
 from .linear import EXL3Linear, EXL3SiblingGroup
+from .paged import PagedBatch, PagedKVCache, check_paged_status, paged_attn, paged_qkv_post
+from .speculative import verify_drafts
 
 __all__ = ["MAX_GEMV_ROWS", "TrellisGemvPlan", "decode_wt", "had_svh", "norm_rot", "rot", "swiglu_rot",
-           "EXL3Linear", "EXL3SiblingGroup"]
+           "EXL3Linear", "EXL3SiblingGroup", "PagedBatch", "PagedKVCache", "check_paged_status", "paged_attn",
+           "paged_qkv_post", "verify_drafts"]

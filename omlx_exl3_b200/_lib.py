@@ -56,11 +56,21 @@ class QkvPostArgs(ctypes.Structure):
                 ("hkv", ctypes.c_int32), ("max_len", ctypes.c_int32), ("eps", ctypes.c_float)]
 
 
+class PagedDesc(ctypes.Structure):
+    """exl3_paged_desc: the pages of one layer and the batch's device tables."""
+    _fields_ = [("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+                ("cu_rows", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("seqs", ctypes.c_int32),
+                ("rows", ctypes.c_int32), ("table_cols", ctypes.c_int32), ("num_pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("hkv", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("dtype", ctypes.c_int32)]
+
+
 _lib = None
 _lock = threading.Lock()
 
 # Every symbol include/exl3_b200.h declares: name -> (restype, argtypes)
 _P, _I, _F, _SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+_LL, _PAGED = ctypes.c_longlong, ctypes.POINTER(PagedDesc)
 SIGNATURES = {
     "exl3_strerror": (ctypes.c_char_p, [_I]),
     "exl3_version": (_I, []),
@@ -97,6 +107,11 @@ SIGNATURES = {
     "exl3_gemv_swiglu": (_I, [ctypes.POINTER(GemvDesc), _P, _I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "exl3_gemv_swiglu_peer": (_I, [ctypes.POINTER(GemvDesc), _P, _I, _P, _P, _P, _P, _P, _P, _SZ,
                                    ctypes.POINTER(PeerGroupDesc), _I, _P]),
+    "exl3_paged_qkv_post": (_I, [_PAGED, _P, _P, _P, _LL, _LL, _LL, _I, _I, _P, _P, _F, _P, _P, _I, _I, _P, _P, _P]),
+    "exl3_paged_attn_workspace": (_I, [_PAGED, _I, ctypes.POINTER(_SZ)]),
+    "exl3_paged_attn": (_I, [_PAGED, _P, _LL, _I, _F, _P, _P, _SZ, _P, _P]),
+    "exl3_verify_workspace": (_I, [_I, _I, _I, ctypes.POINTER(_SZ)]),
+    "exl3_verify_drafts": (_I, [_P, _LL, _P, _LL, _I, _I, _I, _I, _P, _P, _P, _P, _P, _LL, _I, _P, _P, _P, _P, _SZ, _P]),
 }
 
 
