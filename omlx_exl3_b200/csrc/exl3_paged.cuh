@@ -15,13 +15,13 @@ enum : uint32_t { kStatusPagedRange = 8u };
 
 // The sequence of `row`: the first s with row < cu_rows[s + 1], found by the whole warp with 32 probes a
 // round (one round up to 32 sequences, two up to 1024). seqs >= 1 and row < cu_rows[seqs].
-__device__ __forceinline__ int seq_of_row(const int32_t* __restrict__ cu_rows, int seqs, int row, int lane)
+__device__ __forceinline__ int seq_of_row(const int32_t* cu_rows, int seqs, int row, int lane)
 {
     int lo = 0, n = seqs;                                // the answer is in [lo, lo + n)
     while (n > 1) {
         const int step = (n + 31) >> 5;                  // probe the last sequence of each of 32 parts
         const int probe = min(lo + (lane + 1) * step, lo + n);
-        const unsigned past = __ballot_sync(0xffffffffu, __ldg(cu_rows + probe) <= row);
+        const unsigned past = __ballot_sync(0xffffffffu, cu_rows[probe] <= row);
         const int part = min(__popc(past), 31);
         const int end = lo + n;
         lo = min(lo + part * step, end - 1);
@@ -35,7 +35,7 @@ __device__ __forceinline__ int page_of(const exl3_paged_desc& b, int s, int pos)
 {
     const int col = pos / b.page_size;
     if (pos < 0 || col >= b.table_cols) return -1;
-    const int page = __ldg(b.page_table + (size_t)s * b.table_cols + col);
+    const int page = b.page_table[(size_t)s * b.table_cols + col];
     return page >= 0 && page < b.num_pages ? page : -1;
 }
 

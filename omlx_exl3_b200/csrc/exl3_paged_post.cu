@@ -26,7 +26,7 @@ template <typename T>
 __device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8])
 {
     if (vec) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
         const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
@@ -70,10 +70,10 @@ __global__ void __launch_bounds__(128) paged_post_kernel(const PagedPostArgs a)
     float co[8] = {}, si[8] = {};
     if (rotated && !pad && known) {
         const size_t at = (size_t)pos * R + (c0 < R ? c0 : c0 - R);
-        *reinterpret_cast<float4*>(co) = __ldg(reinterpret_cast<const float4*>(a.cos_t + at));
-        *reinterpret_cast<float4*>(co + 4) = __ldg(reinterpret_cast<const float4*>(a.cos_t + at + 4));
-        *reinterpret_cast<float4*>(si) = __ldg(reinterpret_cast<const float4*>(a.sin_t + at));
-        *reinterpret_cast<float4*>(si + 4) = __ldg(reinterpret_cast<const float4*>(a.sin_t + at + 4));
+        *reinterpret_cast<float4*>(co) = *reinterpret_cast<const float4*>(a.cos_t + at);
+        *reinterpret_cast<float4*>(co + 4) = *reinterpret_cast<const float4*>(a.cos_t + at + 4);
+        *reinterpret_cast<float4*>(si) = *reinterpret_cast<const float4*>(a.sin_t + at);
+        *reinterpret_cast<float4*>(si + 4) = *reinterpret_cast<const float4*>(a.sin_t + at + 4);
     }
     const int partner = c0 < R ? lane + R / 8 : lane - R / 8;
     const int heads = a.hq + 2 * b.hkv;
