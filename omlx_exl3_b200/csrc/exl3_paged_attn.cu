@@ -37,19 +37,17 @@
 #include "exl3_common.cuh"
 #include "exl3_host.h"
 #include "exl3_paged.cuh"
+#include "exl3_paged_sched.cuh"
 #include "exl3_tc.cuh"
 
 namespace exl3 {
 
-constexpr int kPaRows = 128;                          // packed query rows of a tile, and TMEM lanes
-constexpr int kPaStep = 128;                          // positions of a step
 constexpr int kPaThreads = 384;                       // two softmax warpgroups; one with the load and the MMA warp
 // Registers of a softmax thread (a row's 128 scores stay in registers) and of the others: 2 x 200 + 104 = 3 x 168, what the
 // launch gives the three warpgroups together.
 constexpr int kPaSoftmaxRegs = 200, kPaOtherRegs = 104;
 constexpr int kPaBarBytes = 512;
 constexpr uint64_t kPaExitNs = 100000000ull;          // wait for a CTA's own copies and MMAs before it exits
-constexpr float kPaSlack = 8.0f;                      // log2 growth of a row's maximum before its accumulator is rescaled
 
 template <int HD>
 struct PaShape {
@@ -59,146 +57,7 @@ struct PaShape {
     static constexpr int kStages = HD == 128 ? 5 : 8;
     static constexpr int kMl = kPaRows * 8;           // slot 1's (m, l) for the merge of a one-tile item
     static constexpr int kSmem = 1024 + 2 * kTile + kStages * kTile + kMl + kPaBarBytes;
-    static constexpr size_t kPart = (size_t)kPaRows * HD * 4 + kPaRows * 8;   // partial O and (m, l) of one tile
     static_assert(kSmem <= 227 * 1024, "shared memory");
-};
-
-struct PaArgs {
-    exl3_paged_desc b;
-    void* out;
-    uint32_t* counters;                               // [CTAs][2] arrivals of the item that starts in the CTA and leaves it
-    uint8_t* parts;                                   // [CTAs][2: began before this CTA, begins in it][2 tiles]
-    uint32_t* status;
-    float scale_log2;
-    int hq, grp, tokens;                              // tokens of a tile
-};
-
-// ------------------------------------------------------------------------------ schedule
-struct PaSeg {
-    int s, h, row0, pos0, ntok[2], rows_used[2];      // sequence, kv head, first row and its position, tokens / rows of the tiles
-    int j0, j1, units, end;                           // this CTA's steps of the item, all of them, first position past the last row
-    bool dual;
-    int c0, c1;                                       // the CTAs that share the item
-};
-
-struct PaSched {
-    const PaArgs& a;
-    long long total, u, left;
-    int ctas, s, h, t, j, cap;
-
-    __device__ __forceinline__ explicit PaSched(const PaArgs& args) : a(args) {}
-
-    __device__ __forceinline__ int item_end(int rows, int len, int t) const
-    {
-        const long long e = (long long)len - rows + min(rows, (t + 1) * 2 * a.tokens);
-        return (int)max(0ll, min(e, (long long)cap));
-    }
-    __device__ __forceinline__ static int units_of(int end) { return max(1, (end + kPaStep - 1) / kPaStep); }
-
-    __device__ __forceinline__ long long seq_units(int q) const
-    {
-        const int rows = q < a.b.seqs ? a.b.cu_rows[q + 1] - a.b.cu_rows[q] : 0;
-        if (rows <= 0) return 0;
-        const int len = a.b.lens[q];
-        long long n = 0;
-        const int items = (rows + 2 * a.tokens - 1) / (2 * a.tokens);
-        for (int i = 0; i < items; ++i) n += units_of(item_end(rows, len, i));
-        return n * a.b.hkv;
-    }
-
-    // All lanes of the warp. This CTA's share of the list, and where it starts.
-    __device__ __forceinline__ void start(int cta, int grid, int lane)
-    {
-        cap = a.b.table_cols * a.b.page_size;
-        long long first = 0;                          // this lane's units of the first 32 sequences
-        total = 0;
-        for (int q0 = 0; q0 < a.b.seqs; q0 += 32) {
-            long long n = seq_units(q0 + lane);
-            if (q0 == 0) first = n;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-            total += n;
-        }
-        s = h = t = j = 0;
-        left = 0;
-        u = 0;
-        ctas = (int)min((long long)grid, total);
-        if (cta >= ctas) return;
-        u = total * cta / ctas;
-        left = total * (cta + 1) / ctas - u;
-        long long before = 0, at = 0;
-        for (int q0 = 0; q0 < a.b.seqs; q0 += 32) {
-            const long long n = q0 == 0 ? first : seq_units(q0 + lane);
-            long long sum = n;                        // inclusive prefix
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long v = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += v;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, before + sum <= u);
-            const int k = __popc(past);
-            if (k < 32) {
-                s = q0 + k;
-                at = u - before - (__shfl_sync(0xffffffffu, sum, k) - __shfl_sync(0xffffffffu, n, k));
-                const long long per = __shfl_sync(0xffffffffu, n, k) / a.b.hkv;
-                h = (int)(at / per);
-                at -= per * h;
-                break;
-            }
-            before += __shfl_sync(0xffffffffu, sum, 31);
-        }
-        const int rows = a.b.cu_rows[s + 1] - a.b.cu_rows[s], len = a.b.lens[s];
-        for (;;) {
-            const int n = units_of(item_end(rows, len, t));
-            if (at < n) break;
-            at -= n;
-            ++t;
-        }
-        j = (int)at;
-    }
-
-    __device__ __forceinline__ int cta_of(long long unit) const { return (int)(((unit + 1) * ctas - 1) / total); }
-
-    // The next segment of this CTA's share; false when it is done.
-    __device__ __forceinline__ bool next(PaSeg& g)
-    {
-        if (left <= 0) return false;
-        const int start_row = a.b.cu_rows[s];
-        const int rows = a.b.cu_rows[s + 1] - start_row, len = a.b.lens[s];
-        const int tok0 = t * 2 * a.tokens, ntok = min(rows - tok0, 2 * a.tokens);
-        g.s = s;
-        g.h = h;
-        g.row0 = start_row + tok0;
-        g.pos0 = (int)max(-(1ll << 30), (long long)len - rows + tok0);
-        g.dual = ntok > a.tokens;
-        g.ntok[0] = min(ntok, a.tokens);
-        g.ntok[1] = ntok - g.ntok[0];
-        g.rows_used[0] = g.ntok[0] * a.grp;
-        g.rows_used[1] = g.ntok[1] * a.grp;
-        g.end = item_end(rows, len, t);
-        g.units = units_of(g.end);
-        g.j0 = j;
-        g.j1 = (int)min((long long)g.units, j + left);
-        g.c0 = cta_of(u - j);
-        g.c1 = cta_of(u - j + g.units - 1);
-        const int n = g.j1 - g.j0;
-        left -= n;
-        u += n;
-        j = 0;
-        if (left > 0) {
-            if (tok0 + 2 * a.tokens < rows) {
-                ++t;
-            } else {
-                t = 0;
-                if (++h == a.b.hkv) {
-                    h = 0;
-                    do ++s;
-                    while (s < a.b.seqs - 1 && a.b.cu_rows[s + 1] <= a.b.cu_rows[s]);
-                }
-            }
-        }
-        return true;
-    }
 };
 
 // ------------------------------------------------------------------------------ instructions
@@ -246,32 +105,10 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16])
         : "memory");
 }
 
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-template <typename C>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi)
-{
-    uint32_t r;
-    if constexpr (std::is_same<C, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
 // Bounded wait of a whole warp, with one answer for all its lanes.
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, uint64_t limit_ns = 2000000000ull)
 {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, limit_ns));
-}
-
-// exp2((m - top) * c), 0 for a row that has seen nothing (m = -inf).
-__device__ __forceinline__ float pa_weight(float m, float top, float c)
-{
-    return m == -INFINITY ? 0.f : ex2((m - top) * c);
 }
 
 // ------------------------------------------------------------------------------ kernel
@@ -296,7 +133,6 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     uint64_t* o_full = p_full + 2;                    // [2] the slot's accumulator is complete
     uint64_t* o_empty = o_full + 2;                   // [2] it has been read
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
-    uint32_t* last_flag = tmem_slot + 1;              // [2]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -329,6 +165,19 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     PaSeg g{};
     bool ok = true;
 
+    // Tiles of the segment: tokens per tile, the second tile's only where the item has more than one tile's.
+    const int tokens = kPaRows / a.grp;
+    struct Item { int row0, pos0, ntok[2]; bool dual; };
+    auto item_of = [&](const PaSeg& g) {
+        const int tok0 = g.p0 / a.grp, ntok = min(g.rows - tok0, 2 * tokens);
+        Item i;
+        i.row0 = g.start + tok0;
+        i.pos0 = g.ctx + tok0;
+        i.dual = ntok > tokens;
+        i.ntok[0] = min(ntok, tokens);
+        i.ntok[1] = ntok - i.ntok[0];
+        return i;
+    };
     if (warp >= 8) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPaOtherRegs));
       if (warp == 8) {
@@ -363,18 +212,19 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         };
         while (ok && sched.next(g)) {
             if (n_seg > 0 && !pa_wait(q_empty, (n_seg - 1) & 1)) { ok = false; break; }
+            const Item im = item_of(g);
             if (lane == 0) {
-                if ((long long)g.pos0 + g.ntok[0] + g.ntok[1] > sched.cap) atomicOr(a.status, kStatusPagedRange);
-                const int tiles = g.dual ? 2 : 1;
-                mbar_arrive_expect_tx(q_full, tiles * P::kPanels * a.tokens * a.grp * 128);
+                if ((long long)im.pos0 + im.ntok[0] + im.ntok[1] > sched.cap) atomicOr(a.status, kStatusPagedRange);
+                const int tiles = im.dual ? 2 : 1;
+                mbar_arrive_expect_tx(q_full, tiles * P::kPanels * tokens * a.grp * 128);
                 for (int i = 0; i < tiles; ++i)
                     for (int p = 0; p < P::kPanels; ++p)
-                        tma_load_3d(q_s + i * P::kTile + p * P::kPanel, &qmap, p * 64, g.h * a.grp, g.row0 + i * a.tokens,
+                        tma_load_3d(q_s + i * P::kTile + p * P::kPanel, &qmap, p * 64, g.h * a.grp, im.row0 + i * tokens,
                                     q_full);
             }
             __syncwarp();
             ++n_seg;
-            const int n = g.j1 - g.j0, ahead = g.dual ? 1 : 2;
+            const int n = g.j1 - g.j0, ahead = im.dual ? 1 : 2;
             int pg0 = page_at(g.j0), pg1 = page_at(g.j0 + 1), pg2 = page_at(g.j0 + 2);   // of steps m, m + 1, m + 2
             load(&kmap, g.j0, pg0);
             if (ahead == 2 && n > 1) load(&kmap, g.j0 + 1, pg1);
@@ -387,6 +237,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                 pg2 = pg3;
             }
         }
+        if (lane == 0) pa_record(a, n_seg > 0, g, n_seg > 0 ? min(2 * tokens, g.rows - g.p0 / a.grp) * a.grp : 0, tokens * a.grp);
         // nothing of this CTA may still be landing when it exits
         for (uint32_t i = it > (uint32_t)P::kStages ? it - P::kStages : 0; i < it; ++i)
             if (!pa_wait(&full[i % P::kStages], (i / P::kStages) & 1, kPaExitNs)) ok = false;
@@ -445,7 +296,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
             if (!pa_wait(q_full, n_seg & 1)) { ok = false; break; }
             ++n_seg;
             const int n = g.j1 - g.j0;
-            if (g.dual) {
+            if (item_of(g).dual) {
                 const uint8_t* k = stage_wait(it);
                 mma_s(0, 0, k);
                 mma_s(1, 1, k);
@@ -509,28 +360,29 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         // ---------------------------------------------------------------- softmax and epilogue
         const int slot = warp >> 2, quarter = warp & 3;
         const int r = quarter * 32 + lane;                             // this thread's row and TMEM lane
-        const int wtid = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_t = tmem + lanes + slot * kPaStep, o_t = tmem + lanes + 256 + slot * HD;
         const float c = a.scale_log2;
         uint32_t n_s = 0, n_o = 0;
         // A wait that gave up only clears ok: the warps stay in step with each other, since they meet at barriers.
         while (sched.next(g)) {
-            const int tile = g.dual ? slot : 0;
-            const int used = g.rows_used[tile];
+            const Item im = item_of(g);
+            const bool dual = im.dual;
+            const int tile = dual ? slot : 0;
+            const int used = im.ntok[tile] * a.grp;
             const int tok = r / a.grp;
-            const int pos = g.pos0 + tile * a.tokens + tok;
+            const int pos = im.pos0 + tile * tokens + tok;
             const int limit = r < used ? min(pos + 1, g.end) : 0;      // positions this row sees
             const bool idle = quarter * 32 >= used;                    // no row of this warp is used
             float m = -INFINITY, l = 0.f;
             const int n = g.j1 - g.j0;
-            const int mine = g.dual ? n : (n + 1 - slot) / 2;
+            const int mine = dual ? n : (n + 1 - slot) / 2;
             for (int i = 0; i < mine; ++i) {
                 if (ok && !pa_wait(&s_full[slot], n_s & 1)) ok = false;
                 ++n_s;
                 tc_fence_after();
                 if (!idle) {
-                    const int step = g.j0 + (g.dual ? i : 2 * i + slot);
+                    const int step = g.j0 + (dual ? i : 2 * i + slot);
                     float x[kPaStep];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) tc_ld32(s_t + q * 32, *reinterpret_cast<float(*)[32]>(x + q * 32));
@@ -602,21 +454,20 @@ __global__ void __launch_bounds__(kPaThreads, 1)
             // The accumulator, 32 columns at a time. In a one-tile item slot 1's steps of the same rows join slot 0's
             // through the free Q tile, half of the columns at a time.
             float4* buf = reinterpret_cast<float4*>(q_s + P::kTile) + r;
-            const bool whole = g.c0 == g.c1;                           // the whole item is this CTA's
-            const int row = g.row0 + tile * a.tokens + tok;
+            const bool whole = g.j0 == 0 && g.j1 == g.units;           // the whole item is this CTA's
+            const int row = im.row0 + tile * tokens + tok;
             const bool live = r < used && row < a.b.rows;
             C* dst = static_cast<C*>(a.out) + ((size_t)row * a.hq + g.h * a.grp + (r - tok * a.grp)) * HD;
-            // this CTA's part of a shared item: [column quad][used row], then (m, l) per row
-            auto part = [&](int cta) { return a.parts + ((size_t)(cta * 2 + (cta == g.c0 ? 1 : 0)) * 2 + tile) * P::kPart; };
-            float4* pdst = reinterpret_cast<float4*>(part(blockIdx.x)) + r;
-            const bool joins = !g.dual && n > 1;                       // slot 1 had steps
-            if (!g.dual && slot == 1) ml_s[r] = make_float2(m, l);
+            uint8_t* part = pa_part<HD, kPaRows, 2>(a.parts, g.c0, blockIdx.x, tile);
+            float4* pdst = reinterpret_cast<float4*>(part) + r;
+            const bool joins = !dual && n > 1;                       // slot 1 had steps
+            if (!dual && slot == 1) ml_s[r] = make_float2(m, l);
             float f0 = 1.f, f1 = 0.f, inv = 0.f;
 #pragma unroll 1
             for (int ch = 0; ch < HD / 32; ++ch) {
                 constexpr int kHalf = HD / 64;                         // chunks of a half
-                const bool sends = !g.dual && slot == 1;
-                if (!g.dual && slot == 0 && ch % kHalf == 0) named_bar_sync(1, 256);
+                const bool sends = !dual && slot == 1;
+                if (!dual && slot == 0 && ch % kHalf == 0) named_bar_sync(1, 256);
                 if (slot == 0 && joins && ch == 0) {
                     const float2 w = ml_s[r];
                     const float top = fmaxf(m, w.x);
@@ -665,7 +516,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                     }
                 }
                 if (sends && ch % kHalf == kHalf - 1) named_bar_sync(1, 256);
-                if (!g.dual && ch % kHalf == kHalf - 1) named_bar_sync(2, 256);
+                if (!dual && ch % kHalf == kHalf - 1) named_bar_sync(2, 256);
             }
             tc_fence_before();
             fence_proxy_async_smem();                                  // the merge buffer is a TMA destination again
@@ -674,50 +525,8 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                 if (mine > 0) mbar_arrive(&o_empty[slot]);
                 mbar_arrive(q_empty);
             }
-            if (whole || (!g.dual && slot == 1)) continue;
-            if (r < used) __stcg(reinterpret_cast<float2*>(part(blockIdx.x) + (size_t)kPaRows * HD * 4) + r, make_float2(m, l));
-            __threadfence();
-            named_bar_sync(3 + slot, 128);
-            if (wtid == 0) {
-                uint32_t* cnt = a.counters + g.c0 * 2 + tile;
-                const bool last = atomicAdd(cnt, 1u) == (uint32_t)(g.c1 - g.c0);
-                if (last) *cnt = 0u;                                   // zero at rest
-                __threadfence();
-                last_flag[slot] = last;
-            }
-            named_bar_sync(3 + slot, 128);
-            const bool last = last_flag[slot] != 0u;
-            named_bar_sync(3 + slot, 128);                             // read before the next item writes it
-            if (!last) continue;
-            __threadfence();
-            for (int e = wtid; e < used * (HD / 4); e += 128) {
-                const int er = e % used, q = e / used;
-                float top = -INFINITY;
-                for (int k = g.c0; k <= g.c1; ++k)
-                    top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(part(k) + (size_t)kPaRows * HD * 4) + er).x);
-                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                float sum = 0.f;
-#pragma unroll 4
-                for (int k = g.c0; k <= g.c1; ++k) {
-                    const uint8_t* pt = part(k);
-                    const float2 w = __ldcg(reinterpret_cast<const float2*>(pt + (size_t)kPaRows * HD * 4) + er);
-                    const float4 y = __ldcg(reinterpret_cast<const float4*>(pt) + e);
-                    const float f = pa_weight(w.x, top, c);
-                    sum += w.y * f;
-                    acc.x += y.x * f;
-                    acc.y += y.y * f;
-                    acc.z += y.z * f;
-                    acc.w += y.w * f;
-                }
-                const int et = er / a.grp, erow = g.row0 + tile * a.tokens + et;
-                if (erow < a.b.rows) {
-                    const float einv = 1.f / sum;
-                    uint2 w = make_uint2(pack2<C>(acc.x * einv, acc.y * einv), pack2<C>(acc.z * einv, acc.w * einv));
-                    if (sum == 0.f) w = make_uint2(0, 0);
-                    *reinterpret_cast<uint2*>(static_cast<C*>(a.out) +
-                                              ((size_t)erow * a.hq + g.h * a.grp + (er - et * a.grp)) * HD + q * 4) = w;
-                }
-            }
+            if (whole || (!dual && slot == 1)) continue;
+            if (r < used) __stcg(reinterpret_cast<float2*>(part + PaPart<HD, kPaRows>::kMl) + r, make_float2(m, l));
         }
     }
     if (!ok && lane == 0) atomicOr(a.status, kStatusPipeTimeout);
@@ -765,17 +574,33 @@ static bool pa_map_q(PFN_cuTensorMapEncodeTiled_v12000 encode, CUtensorMap* map,
 static int check_attn(const exl3_paged_desc* b, int hq)
 {
     if (int e = exl3_check_paged(b)) return e;
-    if (hq < 1 || hq % b->hkv || hq / b->hkv > kPaRows) return EXL3_E_SHAPE;
+    if (hq < 1 || hq % b->hkv || hq / b->hkv > kPaRows || (long long)b->rows * hq > 0x7fffffffll) return EXL3_E_SHAPE;
     return EXL3_OK;
 }
 
-static int attn_ctas() { return std::min(device_sm_count(), EXL3_PAGED_HEADER_BYTES / 8); }
+static int attn_ctas() { return device_sm_count(); }
+
+// Workspace: the two kernels' items, the tiles' parts, the few rows' parts.
+struct AttnSpace {
+    size_t few_items, tile_parts, few_parts, bytes;
+};
 
 template <int HD>
-static size_t attn_bytes() { return EXL3_PAGED_HEADER_BYTES + (size_t)attn_ctas() * 4 * PaShape<HD>::kPart; }
+static AttnSpace attn_space()
+{
+    const size_t n = attn_ctas();
+    AttnSpace w;
+    w.few_items = n * sizeof(PaItem);
+    w.tile_parts = (2 * n * sizeof(PaItem) + 255) / 256 * 256;
+    w.few_parts = w.tile_parts + n * 4 * PaPart<HD, kPaRows>::kBytes;
+    w.bytes = w.few_parts + n * 2 * PaPart<HD, kPaFew>::kBytes;
+    return w;
+}
+
+static AttnSpace attn_space(const exl3_paged_desc& b) { return b.head_dim == 128 ? attn_space<128>() : attn_space<64>(); }
 
 template <typename C, int HD>
-static int launch_attn(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const PaArgs& a, cudaStream_t s)
+static int launch_tiles(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const PaArgs& a, cudaStream_t s)
 {
     static bool attr_set[64] = {false};
     int dev = 0;
@@ -789,6 +614,24 @@ static int launch_attn(const CUtensorMap& qm, const CUtensorMap& km, const CUten
     return launch_pdl(paged_attn_kernel<C, HD>, dim3(attn_ctas()), dim3(kPaThreads), PaShape<HD>::kSmem, s, qm, km, vm, a);
 }
 
+int pa_launch_tiles(const PaArgs& args, cudaStream_t s)
+{
+    PaArgs a = args;
+    const int tokens = kPaRows / a.grp;
+    a.span = 2 * tokens * a.grp;
+    a.item = getenv("PT_ITEM") ? atoi(getenv("PT_ITEM")) : 2;
+    auto encode = exl3_get_tensormap_encoder();
+    if (!encode) return EXL3_E_CUDA;
+    CUtensorMap qm, km, vm;
+    if (!pa_map_q(encode, &qm, a.q, a.q_stride, a.b, a.hq, a.grp, tokens) || !pa_map_pages(encode, &km, a.b.k_pages, a.b) ||
+        !pa_map_pages(encode, &vm, a.b.v_pages, a.b))
+        return EXL3_E_CUDA;
+    if (a.b.dtype == EXL3_F16)
+        return a.b.head_dim == 128 ? launch_tiles<__half, 128>(qm, km, vm, a, s) : launch_tiles<__half, 64>(qm, km, vm, a, s);
+    return a.b.head_dim == 128 ? launch_tiles<__nv_bfloat16, 128>(qm, km, vm, a, s)
+                               : launch_tiles<__nv_bfloat16, 64>(qm, km, vm, a, s);
+}
+
 }  // namespace exl3
 
 using namespace exl3;
@@ -797,7 +640,8 @@ extern "C" int exl3_paged_attn_workspace(const exl3_paged_desc* batch, int hq, s
 {
     if (!bytes) return EXL3_E_NULL;
     if (int e = check_attn(batch, hq)) return e;
-    *bytes = batch->head_dim == 128 ? attn_bytes<128>() : attn_bytes<64>();
+    if (int e = check_device()) return e;
+    *bytes = attn_space(*batch).bytes;
     return EXL3_OK;
 }
 
@@ -808,29 +652,39 @@ extern "C" int exl3_paged_attn(const exl3_paged_desc* batch, const void* q, long
     if (batch->rows == 0) return EXL3_OK;
     if (!q || !out || !status || !workspace) return EXL3_E_NULL;
     if (q_stride < (long long)hq * batch->head_dim || !(scale > 0.f)) return EXL3_E_SHAPE;
-    if (!aligned(q, 16) || !aligned(out, 16) || !aligned(status, 4) || !aligned(workspace, 16) || q_stride % 8)
+    if (!aligned(q, 16) || !aligned(out, 16) || !aligned(status, 4) || !aligned(workspace, 256) || q_stride % 8)
         return EXL3_E_ALIGN;
     if (int e = check_device()) return e;
-    if (workspace_bytes < (batch->head_dim == 128 ? attn_bytes<128>() : attn_bytes<64>())) return EXL3_E_WORKSPACE;
-    auto encode = exl3_get_tensormap_encoder();
-    if (!encode) return EXL3_E_CUDA;
+    const AttnSpace w = attn_space(*batch);
+    if (workspace_bytes < w.bytes) return EXL3_E_WORKSPACE;
     PaArgs a{};
     a.b = *batch;
+    a.q = q;
+    a.q_stride = q_stride;
     a.out = out;
-    a.counters = static_cast<uint32_t*>(workspace);
-    a.parts = static_cast<uint8_t*>(workspace) + EXL3_PAGED_HEADER_BYTES;
     a.status = status;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.hq = hq;
     a.grp = hq / batch->hkv;
-    a.tokens = kPaRows / a.grp;
-    CUtensorMap qm, km, vm;
-    if (!pa_map_q(encode, &qm, q, q_stride, *batch, hq, a.grp, a.tokens) || !pa_map_pages(encode, &km, batch->k_pages, *batch) ||
-        !pa_map_pages(encode, &vm, batch->v_pages, *batch))
-        return EXL3_E_CUDA;
+    // Which kernel takes a sequence goes by its packed rows, which only the device knows, unless there is one sequence. A
+    // batch with a row per sequence at most is taken for single tokens: one launch, right whatever the rows are.
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (batch->dtype == EXL3_F16)
-        return batch->head_dim == 128 ? launch_attn<__half, 128>(qm, km, vm, a, s) : launch_attn<__half, 64>(qm, km, vm, a, s);
-    return batch->head_dim == 128 ? launch_attn<__nv_bfloat16, 128>(qm, km, vm, a, s)
-                                  : launch_attn<__nv_bfloat16, 64>(qm, km, vm, a, s);
+    const bool few_only = a.grp <= kPaFew && (batch->seqs == 1 ? (long long)batch->rows * a.grp <= kPaFew
+                                                               : batch->rows <= batch->seqs);
+    const bool tiles_only = !few_only && (batch->seqs == 1 || a.grp > kPaFew);
+    uint8_t* base = static_cast<uint8_t*>(workspace);
+    PaArgs few = a, tiles = a;
+    few.items = reinterpret_cast<PaItem*>(base + w.few_items);
+    few.parts = base + w.few_parts;
+    few.lo = 0;
+    few.hi = few_only ? 0x7fffffff : kPaFew;
+    tiles.items = reinterpret_cast<PaItem*>(base);
+    tiles.parts = base + w.tile_parts;
+    tiles.lo = tiles_only ? 0 : kPaFew;
+    tiles.hi = 0x7fffffff;
+    if (!tiles_only)
+        if (int e = pa_launch_few(few, s)) return e;
+    if (!few_only)
+        if (int e = pa_launch_tiles(tiles, s)) return e;
+    return pa_launch_merge(few_only ? nullptr : &tiles, tiles_only ? nullptr : &few, attn_ctas(), s);
 }

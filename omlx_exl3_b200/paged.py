@@ -27,7 +27,6 @@ import torch
 from . import _lib
 from ._lib import PagedDesc, check, dtype_code, lib, stream_ptr
 
-HEADER_BYTES = 4096           # arrival counters at the start of paged_attn's workspace (EXL3_PAGED_HEADER_BYTES)
 _CACHE_DTYPES = (torch.float16, torch.bfloat16)
 _status: dict = {}
 _workspaces: dict = {}
@@ -148,17 +147,14 @@ def paged_qkv_post(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm_w: 
     return q_out
 
 
-def _workspace(device: torch.device, stream: int, nbytes: int, header: int) -> torch.Tensor:
-    """Scratch of this device and stream whose first `header` bytes (arrival counters) are zero at rest: calls on
-    different streams may overlap, calls on one stream run one after another. A captured call gets scratch of its own
-    from the graph's pool, its counters zeroed by a node of the graph: replays may run beside eager calls."""
+def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+    """Scratch of this device and stream: calls on different streams may overlap, calls on one stream run one after
+    another. A captured call gets scratch of its own from the graph's pool: replays may run beside eager calls."""
     if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        ws[:header].zero_()
-        return ws
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     ws = _workspaces.get((device.index, stream))
     if ws is None or ws.numel() < nbytes:
-        ws = _workspaces[(device.index, stream)] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        ws = _workspaces[(device.index, stream)] = torch.empty(nbytes, dtype=torch.uint8, device=device)
     return ws
 
 
@@ -194,7 +190,7 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
         stream = stream_ptr(dev)
         need = ctypes.c_size_t()
         check(lib().exl3_paged_attn_workspace(b, hq, ctypes.byref(need)), "exl3_paged_attn_workspace")
-        ws = _workspace(dev, stream, need.value, HEADER_BYTES)
+        ws = _workspace(dev, stream, need.value)
         check(lib().exl3_paged_attn(b, q.data_ptr(), q.stride(0), hq, scale, out.data_ptr(), ws.data_ptr(), ws.numel(),
                                     _status_word(dev).data_ptr(), stream), "exl3_paged_attn")
     return out

@@ -65,7 +65,7 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, cu_ro
         stream = stream_ptr(dev)
         need = ctypes.c_size_t()
         check(lib().exl3_verify_workspace(rows, seqs, n, ctypes.byref(need)), "exl3_verify_workspace")
-        ws = _workspace(dev, stream, need.value, need.value)
+        ws = _workspace(dev, stream, need.value)
         check(lib().exl3_verify_drafts(target_logits.data_ptr(), max(target_logits.stride(0), n),
                                        None if draft_logits is None or drafts == 0 else draft_logits.data_ptr(),
                                        n if draft_logits is None else max(draft_logits.stride(0), n), code, rows, seqs, n,
