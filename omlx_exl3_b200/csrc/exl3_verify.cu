@@ -1,16 +1,31 @@
 // Verification of drafted tokens against the target's probabilities, from given random numbers.
 //
-//   a_i = min(1, p_i(x_i) / q_i(x_i)), drafts accepted while u_i < a_i, then one draw from max(0, p - q) (after
-//   a rejection) or p as the first largest w(v) / noise(v).
+//   p = softmax(target / T), q = softmax(draft / T); a_i = min(1, p_i(x_i) / q_i(x_i)), drafts accepted while u_i < a_i, then
+//   one draw from w = max(0, p - q) (after a rejection) or w = p, as the first largest w(v) / noise(v).
 //
-// One CTA per sequence: softmax statistics of each row pair in turn, then the race over the chosen row.
+// Two launches, both bound by reading logits (or, for a sequence or two, by latency):
+//   stats    a CTA per chunk of a row keeps it in registers: maximum, sum of exp, and for T = 0 the first column of the
+//            maximum. Rows do not wait for each other and every logit is read once.
+//   decide   a cluster of 8 CTAs per sequence: each works out the acceptances from the statistics (the same answer in all of
+//            them), then they share the columns of the one row that the next token is drawn from and reduce (value, first
+//            column) through distributed shared memory.
+// A draw by inverting the cumulative distribution would need a prefix sum over the vocabulary and give another token for
+// another order of summation; the race depends on each w alone.
 #include <cuda_runtime.h>
 
 #include "exl3_b200.h"
 #include "exl3_common.cuh"
 #include "exl3_host.h"
+#include "exl3_paged.cuh"
+#include "exl3_paged_sched.cuh"
+#include "exl3_tc.cuh"
 
 namespace exl3 {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kVerifyThreads = 512;
+constexpr int kVerifyWarps = kVerifyThreads / 32;
+constexpr int kVerifyCluster = 8;
 
 struct VerifyArgs {
     const void *target, *draft;
@@ -21,148 +36,330 @@ struct VerifyArgs {
     long long* out;
     int32_t* count;
     float* prob;
-    int rows, seqs, n, max_drafts;
+    float4* stats;                                    // [target rows, then draft rows][chunks] (max, sum, first column of max)
+    int rows, seqs, n, max_drafts, chunks;
 };
 
-constexpr int kVerifyThreads = 512;
-
-// (max, first column of the max, sum of exp((x - max) * inv_t)) of a row, the same in every thread.
-template <typename T>
-__device__ void row_stats(const T* x, int n, float inv_t, float& m, int& at, float& sum)
+// The sequence of draft i: sequence s holds drafts cu_rows[s] - s .. cu_rows[s + 1] - s - 2.
+__device__ __forceinline__ int seq_of_draft(const int32_t* cu_rows, int seqs, int i)
 {
-    __shared__ float sm[16];
-    __shared__ int sa[16];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    m = -INFINITY;
-    at = 0x7fffffff;
-    for (int i = threadIdx.x; i < n; i += kVerifyThreads) {
-        const float v = to_f32(x[i]);
-        if (v > m || (v == m && i < at)) { m = v; at = i; }
+    int lo = 0, hi = seqs - 1;                        // the first s with i < cu_rows[s + 1] - s - 1
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (i < cu_rows[mid + 1] - mid - 1) hi = mid;
+        else lo = mid + 1;
     }
+    return lo;
+}
+
+// (value, column) of the larger value, of the first column among equals.
+__device__ __forceinline__ void take_first(float& v, int& i, float ov, int oi)
+{
+    if (ov > v || (ov == v && oi < i)) {
+        v = ov;
+        i = oi;
+    }
+}
+
+// ------------------------------------------------------------------------------ statistics
+// PER columns per thread. The row's columns from its first 16-byte boundary on go to the chunks as whole vectors; the few
+// before it are chunk 0's, the last vector may be partial.
+template <typename T, int PER>
+__global__ void __launch_bounds__(kVerifyThreads) verify_stats_kernel(const VerifyArgs a)
+{
+    constexpr int VEC = 16 / sizeof(T), N = PER / VEC;
+    __shared__ float sv[kVerifyWarps];
+    __shared__ int si[kVerifyWarps];
+    pdl_trigger();
+    pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int r = blockIdx.x / a.chunks, chunk = blockIdx.x - r * a.chunks;
+    const bool is_draft = r >= a.rows;
+    float temp = 1.f;
+    if (a.temperature) {
+        const int s = is_draft ? seq_of_draft(a.cu_rows, a.seqs, r - a.rows) : seq_of_row(a.cu_rows, a.seqs, r, lane);
+        temp = a.temperature[s];
+    }
+    const bool greedy = !(temp > 0.f);
+    if (greedy && is_draft) return;                   // q is one-hot: the row is not looked at
+    const T* x = is_draft ? static_cast<const T*>(a.draft) + (r - a.rows) * a.draft_ld
+                          : static_cast<const T*>(a.target) + r * a.target_ld;
+    const int head = min(a.n, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
+    const int first = head + chunk * (kVerifyThreads * PER) + tid * VEC;
+    float v[PER + 1];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int at = first + k * kVerifyThreads * VEC;
+        if (at + VEC <= a.n) {
+            const uint4 w = *reinterpret_cast<const uint4*>(x + at);
+            const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[k * VEC + i] = to_f32(e[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[k * VEC + i] = at + i < a.n ? to_f32(x[at + i]) : -INFINITY;
+        }
+    }
+    v[PER] = chunk == 0 && tid < head ? to_f32(x[tid]) : -INFINITY;
+    float m = v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) m = fmaxf(m, v[i]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) sv[warp] = m;
+    __syncthreads();
+    m = sv[lane & (kVerifyWarps - 1)];
+#pragma unroll
+    for (int o = kVerifyWarps / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float base = m == -INFINITY ? 0.f : m, c = (greedy ? 1.f : 1.f / temp) * kLog2e;
+    float s0 = ex2((v[PER] - base) * c), s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; i += 2) {
+        s0 += ex2((v[i] - base) * c);
+        s1 += ex2((v[i + 1] - base) * c);
+    }
+    const float s = warp_sum(s0 + s1);
+    int at = 0x7fffffff;
+    if (greedy) {
+#pragma unroll
+        for (int i = PER - 1; i >= 0; --i)
+            if (v[i] == m) at = first + (i / VEC) * kVerifyThreads * VEC + i % VEC;
+        if (chunk == 0 && tid < head && v[PER] == m) at = tid;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
+    }
+    __syncthreads();
+    if (lane == 0) {
+        sv[warp] = s;
+        si[warp] = at;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        float sum = 0.f;
+        int col = 0x7fffffff;
+        for (int w = 0; w < kVerifyWarps; ++w) {
+            sum += sv[w];
+            col = min(col, si[w]);
+        }
+        a.stats[blockIdx.x] = make_float4(m, sum, __int_as_float(col), 0.f);
+    }
+}
+
+// ------------------------------------------------------------------------------ decision
+// What the race needs of a row: exp2((x - m) c) * inv is its probability.
+struct RowStat {
+    float m, inv;
+    int first;                                        // column of the maximum
+};
+
+// Two sums of exp relative to their own maxima, relative to the larger one. A part of -inf alone has sum 0 (or NaN, which
+// stays: its row has no probabilities).
+__device__ __forceinline__ float joined(float s0, float m0, float s1, float m1, float now, float c)
+{
+    return (m0 == -INFINITY ? s0 : s0 * ex2((m0 - now) * c)) + (m1 == -INFINITY ? s1 : s1 * ex2((m1 - now) * c));
+}
+
+__device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, int row, float c, int lane)
+{
+    float m = -INFINITY, s = 0.f;
+    int at = 0x7fffffff;
+    for (int k = lane; k < a.chunks; k += 32) {
+        const float4 w = __ldcg(a.stats + (size_t)row * a.chunks + k);
+        const float now = fmaxf(m, w.x);
+        s = joined(s, m, w.y, w.x, now, c);
+        take_first(m, at, w.x, __float_as_int(w.z));
+    }
+#pragma unroll
     for (int o = 16; o; o >>= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, o);
+        const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o);
         const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-        if (om > m || (om == m && oa < at)) { m = om; at = oa; }
+        const float now = fmaxf(m, om);
+        s = joined(s, m, os, om, now, c);
+        take_first(m, at, om, oa);
     }
-    __syncthreads();
-    if (lane == 0) { sm[warp] = m; sa[warp] = at; }
-    __syncthreads();
-    m = sm[0];
-    at = sa[0];
-    for (int w = 1; w < 16; ++w)
-        if (sm[w] > m || (sm[w] == m && sa[w] < at)) { m = sm[w]; at = sa[w]; }
-    const float base = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
-    for (int i = threadIdx.x; i < n; i += kVerifyThreads) s += expf((to_f32(x[i]) - base) * inv_t);
-    s = warp_sum(s);
-    __syncthreads();
-    if (lane == 0) sm[warp] = s;
-    __syncthreads();
-    sum = 0.f;
-    for (int w = 0; w < 16; ++w) sum += sm[w];
-    m = base;
+    RowStat r;
+    r.m = m == -INFINITY ? 0.f : m;
+    r.inv = s > 0.f ? 1.f / s : 0.f;
+    r.first = at;
+    return r;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a)
+__device__ __forceinline__ float prob_of(const T* x, long long v, const RowStat& r, float c)
 {
-    __shared__ float bv[16];
-    __shared__ int bi[16];
+    return ex2((to_f32(x[v]) - r.m) * c) * r.inv;
+}
+
+struct Verdict {                                      // of one row, by the warp that looked at it
+    RowStat p, q;
+    float prob;
+    long long token;
+    int stands;                                       // its draft was accepted
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kVerifyThreads) verify_decide_kernel(const VerifyArgs a)
+{
+    constexpr int VEC = 16 / sizeof(T);
+    __shared__ Verdict row_s[kVerifyWarps];
+    __shared__ float bv[kVerifyWarps];
+    __shared__ int bi[kVerifyWarps];
+    __shared__ float2 mine[2];                        // this CTA's winner of a pass (value, column)
     pdl_trigger();
     pdl_wait();
-    const int s = blockIdx.x, tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = (int)cluster_rank();
+    const int s = blockIdx.x / kVerifyCluster;
     const int lo = a.cu_rows[s], hi = a.cu_rows[s + 1];
-    long long* out = a.out + (size_t)s * (a.max_drafts + 1);
-    const bool sane = lo >= 0 && hi > lo && hi <= a.rows;
+    const bool sane = lo >= s && hi > lo && hi <= a.rows && hi - s - 1 <= a.rows - a.seqs;
     const float temp = a.temperature ? a.temperature[s] : 1.f;
-    const float inv_t = temp > 0.f ? 1.f / temp : 1.f;
-    const int drafts = sane ? min(hi - lo - 1, a.max_drafts) : 0;
-    int n_acc = 0;
-    bool going = true;
-    float m = 0.f, sum = 0.f, qm = 0.f, qsum = 0.f, w_inv = 0.f, q_inv = 0.f;
-    int at = 0, qat;
-    long long x = -1;
-    bool rejected = false;
-    for (int j = 0; sane && j < hi - lo; ++j) {
-        const bool last = j == hi - lo - 1;
-        if (last && !going) break;
-        const int row = lo + j, i = row - s;
-        float pm, psum;
-        int pat;
-        const T* tr = static_cast<const T*>(a.target) + row * a.target_ld;
-        row_stats(tr, a.n, inv_t, pm, pat, psum);
-        const float p_inv = psum > 0.f ? 1.f / psum : 0.f;
-        if (last || (j >= a.max_drafts && going)) {
-            if (going) { m = pm; at = pat; w_inv = p_inv; n_acc = j; going = false; }
-            if (last) break;
-        }
-        if (i < 0 || i >= a.rows - a.seqs) break;
-        const long long d = a.tokens[i];
-        const bool in = d >= 0 && d < a.n;
-        const T* dr = a.draft ? static_cast<const T*>(a.draft) + i * a.draft_ld : nullptr;
-        float pd = 0.f, qd = 1.f, dm = 0.f, dsum = 0.f, d_inv = 0.f;
-        if (temp > 0.f) {
-            if (in) pd = expf((to_f32(tr[d]) - pm) * inv_t) * p_inv;
-            if (dr) {
-                row_stats(dr, a.n, inv_t, dm, qat, dsum);
-                d_inv = dsum > 0.f ? 1.f / dsum : 0.f;
-                qd = in ? expf((to_f32(dr[d]) - dm) * inv_t) * d_inv : 0.f;
+    const bool greedy = !(temp > 0.f);
+    const float c = (greedy ? 1.f : 1.f / temp) * kLog2e;
+    const int judged = sane ? hi - lo - 1 : 0;        // drafts of this sequence
+    const int limit = min(judged, a.max_drafts);
+
+    // rows in order, a warp each, until one does not stand (the first CTA goes on: accept_prob is every draft's)
+    int n_acc = -1;
+    Verdict at{};
+    for (int j0 = 0; sane && j0 <= judged; j0 += kVerifyWarps) {
+        const int j = j0 + warp;
+        if (j <= judged) {
+            const T* tr = static_cast<const T*>(a.target) + (lo + j) * a.target_ld;
+            Verdict v{};
+            v.p = row_stat(a, lo + j, c, lane);
+            if (j < judged) {
+                const int i = lo + j - s;
+                v.token = a.tokens[i];
+                const bool in = v.token >= 0 && v.token < a.n;
+                float p = 0.f, q = 1.f;
+                if (greedy) {
+                    p = in && v.token == v.p.first && v.p.inv > 0.f ? 1.f : 0.f;
+                } else {
+                    if (in) p = prob_of(tr, v.token, v.p, c);
+                    if (a.draft) {
+                        const T* dr = static_cast<const T*>(a.draft) + i * a.draft_ld;
+                        v.q = row_stat(a, a.rows + i, c, lane);
+                        q = in ? prob_of(dr, v.token, v.q, c) : 0.f;
+                    }
+                }
+                v.prob = q > 0.f ? fminf(p / q, 1.f) : (p > 0.f ? 1.f : 0.f);
+                v.stands = j < limit && a.u[i] < v.prob;
+                if (rank == 0 && lane == 0) a.prob[i] = v.prob;
             }
-        } else {
-            pd = in && d == pat && psum > 0.f ? 1.f : 0.f;
+            if (lane == 0) row_s[warp] = v;
         }
-        const float prob = qd > 0.f ? fminf(pd / qd, 1.f) : (pd > 0.f ? 1.f : 0.f);
-        if (tid == 0) a.prob[i] = prob;
-        if (!going) continue;
-        if (a.u[i] < prob) {
-            if (tid == 0) out[j] = d;
-            continue;
-        }
-        going = false;
-        rejected = true;
-        n_acc = j;
-        m = pm; at = pat; sum = psum; w_inv = p_inv; qm = dm; qsum = dsum; q_inv = d_inv;
-        x = d;
+        __syncthreads();
+        if (n_acc < 0)
+            for (int k = 0; k < kVerifyWarps && j0 + k <= judged; ++k)
+                if (!row_s[k].stands) {
+                    n_acc = j0 + k;
+                    at = row_s[k];
+                    break;
+                }
+        __syncthreads();
+        if (n_acc >= 0 && rank != 0) break;
     }
-    (void)sum; (void)qsum; (void)drafts;
+    const bool rejected = n_acc >= 0 && n_acc < limit;                // the row's own draft was turned down
+
     long long next = -1;
-    if (sane) {
-        if (temp > 0.f) {
-            const T* tr = static_cast<const T*>(a.target) + (lo + n_acc) * a.target_ld;
-            const T* dr = a.draft && rejected ? static_cast<const T*>(a.draft) + (lo + n_acc - s) * a.draft_ld : nullptr;
-            const float* e = a.noise + s * a.noise_ld;
-            for (int pass = rejected ? 0 : 1; pass < 2 && next < 0; ++pass) {
-                float best = 0.f;
-                int idx = 0x7fffffff;
-                for (int v = tid; v < a.n; v += kVerifyThreads) {
-                    float w = expf((to_f32(tr[v]) - m) * inv_t) * w_inv;
-                    if (pass == 0) w -= dr ? expf((to_f32(dr[v]) - qm) * inv_t) * q_inv : (v == x ? 1.f : 0.f);
-                    const float r = w / e[v];
-                    if (r > best) { best = r; idx = v; }
+    if (sane && greedy) {
+        if (at.p.inv > 0.f) next = at.p.first;
+    } else if (sane) {
+        const T* tr = static_cast<const T*>(a.target) + (lo + n_acc) * a.target_ld;
+        const T* dr = a.draft && rejected ? static_cast<const T*>(a.draft) + (lo + n_acc - s) * a.draft_ld : nullptr;
+        const float* e = a.noise + s * a.noise_ld;
+        const bool vec = ((reinterpret_cast<uintptr_t>(tr) | reinterpret_cast<uintptr_t>(dr) | reinterpret_cast<uintptr_t>(e)) & 15) == 0;
+        // first the residual, then (where that is zero everywhere) p itself
+        for (int pass = rejected ? 0 : 1; pass < 2; ++pass) {
+            float best = 0.f;
+            int idx = 0x7fffffff;
+            auto consider = [&](int v, float x, float d, float noise) {
+                float w = ex2((x - at.p.m) * c) * at.p.inv;
+                if (pass == 0) w -= dr ? ex2((d - at.q.m) * c) * at.q.inv : (v == at.token ? 1.f : 0.f);
+                const float score = w / noise;
+                if (score > best) {                   // columns come in rising order per thread
+                    best = score;
+                    idx = v;
                 }
-                for (int o = 16; o; o >>= 1) {
-                    const float ob = __shfl_xor_sync(0xffffffffu, best, o);
-                    const int oi = __shfl_xor_sync(0xffffffffu, idx, o);
-                    if (ob > best || (ob == best && oi < idx)) { best = ob; idx = oi; }
-                }
-                __syncthreads();
-                if ((tid & 31) == 0) { bv[tid >> 5] = best; bi[tid >> 5] = idx; }
-                __syncthreads();
-                best = bv[0];
-                idx = bi[0];
-                for (int w = 1; w < 16; ++w)
-                    if (bv[w] > best || (bv[w] == best && bi[w] < idx)) { best = bv[w]; idx = bi[w]; }
-                if (best > 0.f) next = idx;
+            };
+            const int threads = kVerifyThreads * kVerifyCluster, me = rank * kVerifyThreads + tid;
+            const int whole = vec ? a.n / VEC * VEC : 0;
+            for (int v = me * VEC; v < whole; v += threads * VEC) {
+                const uint4 xr = *reinterpret_cast<const uint4*>(tr + v);
+                const uint4 dx = dr && pass == 0 ? *reinterpret_cast<const uint4*>(dr + v) : make_uint4(0, 0, 0, 0);
+                float4 nz[VEC / 4];
+#pragma unroll
+                for (int i = 0; i < VEC / 4; ++i) nz[i] = *reinterpret_cast<const float4*>(e + v + 4 * i);
+                const T* xe = reinterpret_cast<const T*>(&xr);
+                const T* de = reinterpret_cast<const T*>(&dx);
+                const float* ne = reinterpret_cast<const float*>(nz);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) consider(v + i, to_f32(xe[i]), to_f32(de[i]), ne[i]);
             }
-        } else if (w_inv > 0.f) {
-            next = at;
+#pragma unroll 4
+            for (int v = whole + me; v < a.n; v += threads)
+                consider(v, to_f32(tr[v]), dr && pass == 0 ? to_f32(dr[v]) : 0.f, e[v]);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) take_first(best, idx, __shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, idx, o));
+            if (lane == 0) {
+                bv[warp] = best;
+                bi[warp] = idx;
+            }
+            __syncthreads();
+            if (tid == 0) {
+                for (int w = 1; w < kVerifyWarps; ++w) take_first(best, idx, bv[w], bi[w]);
+                mine[pass] = make_float2(best, __int_as_float(idx));
+            }
+            cluster_sync_all();
+            best = 0.f;
+            idx = 0x7fffffff;
+            for (int k = 0; k < kVerifyCluster; ++k) {
+                float ov;
+                int oi;
+                const uint32_t from = cluster_addr(&mine[pass], k);
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ov) : "r"(from) : "memory");
+                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(oi) : "r"(from + 4) : "memory");
+                take_first(best, idx, ov, oi);
+            }
+            if (best > 0.f) {
+                next = idx;
+                break;
+            }
         }
+        cluster_sync_all();                           // no CTA leaves while another reads its result
     }
-    if (tid == 0) {
-        out[n_acc] = next;
-        for (int j = n_acc + 1; j <= a.max_drafts; ++j) out[j] = -1;
-        a.count[s] = sane ? n_acc + 1 : 0;
+    if (rank == 0) {
+        long long* out = a.out + (size_t)s * (a.max_drafts + 1);
+        for (int j = tid; j <= a.max_drafts; j += kVerifyThreads)
+            out[j] = j < n_acc ? a.tokens[lo + j - s] : j == n_acc ? next : -1;
+        if (tid == 0) a.count[s] = n_acc + 1;
     }
+}
+
+// 32 columns a thread, or 8 where that leaves SMs without a CTA (a sequence or two).
+struct VerifyPlan {
+    int per, chunks;
+    long long stat_rows;
+};
+
+static VerifyPlan verify_plan(int rows, int seqs, int n)
+{
+    VerifyPlan p;
+    p.stat_rows = 2ll * rows - seqs;
+    p.per = p.stat_rows * (n / (32 * kVerifyThreads) + 1) < 2 * device_sm_count() ? 8 : 32;
+    p.chunks = (n + p.per * kVerifyThreads - 1) / (p.per * kVerifyThreads);
+    return p;
+}
+
+template <typename T>
+static int launch_verify(const VerifyArgs& a, int per, cudaStream_t s)
+{
+    const long long ctas = (long long)(a.rows + (a.draft ? a.rows - a.seqs : 0)) * a.chunks;
+    if (ctas > 0x7fffffffll) return EXL3_E_SHAPE;
+    const int e = per == 8 ? launch_pdl(verify_stats_kernel<T, 8>, dim3((unsigned)ctas), dim3(kVerifyThreads), 0, s, a)
+                           : launch_pdl(verify_stats_kernel<T, 32>, dim3((unsigned)ctas), dim3(kVerifyThreads), 0, s, a);
+    if (e) return e;
+    return launch_pdl_cluster(verify_decide_kernel<T>, dim3(a.seqs * kVerifyCluster), dim3(kVerifyThreads), 0, kVerifyCluster, s, a);
 }
 
 }  // namespace exl3
@@ -171,14 +368,15 @@ using namespace exl3;
 
 static int check_verify(int rows, int seqs, int n)
 {
-    return seqs < 1 || rows < seqs || n < 1 ? EXL3_E_SHAPE : EXL3_OK;
+    return seqs < 1 || seqs > (1 << 24) || rows < seqs || rows > (1 << 30) || n < 1 || n > (1 << 30) ? EXL3_E_SHAPE : EXL3_OK;
 }
 
 extern "C" int exl3_verify_workspace(int rows, int seqs, int n, size_t* bytes)
 {
     if (!bytes) return EXL3_E_NULL;
     if (int e = check_verify(rows, seqs, n)) return e;
-    *bytes = 0;
+    const VerifyPlan p = verify_plan(rows, seqs, n);
+    *bytes = (size_t)p.stat_rows * p.chunks * sizeof(float4);
     return EXL3_OK;
 }
 
@@ -189,27 +387,30 @@ extern "C" int exl3_verify_drafts(const void* target, long long target_ld, const
                                   void* workspace, size_t workspace_bytes, void* stream)
 {
     if (int e = check_verify(rows, seqs, n)) return e;
-    if (!target || !cu_rows || !noise || !tokens_out || !count) return EXL3_E_NULL;
+    if (!target || !cu_rows || !noise || !tokens_out || !count || !workspace) return EXL3_E_NULL;
     if (rows > seqs && (!draft_tokens || !u || !accept_prob)) return EXL3_E_NULL;
     if (target_ld < n || (draft && draft_ld < n) || noise_ld < n || max_drafts < 0) return EXL3_E_SHAPE;
     const int esz = dtype == EXL3_F32 ? 4 : 2;
     if (dtype != EXL3_F16 && dtype != EXL3_BF16 && dtype != EXL3_F32) return EXL3_E_DTYPE;
     if (!aligned(target, esz) || !aligned(draft, esz) || !aligned(noise, 4) || !aligned(u, 4) || !aligned(cu_rows, 4) ||
         !aligned(draft_tokens, 8) || !aligned(tokens_out, 8) || !aligned(count, 4) || !aligned(accept_prob, 4) ||
-        !aligned(temperature, 4))
+        !aligned(temperature, 4) || !aligned(workspace, 16))
         return EXL3_E_ALIGN;
     if (int e = check_device()) return e;
+    const VerifyPlan p = verify_plan(rows, seqs, n);
+    if (workspace_bytes < (size_t)p.stat_rows * p.chunks * sizeof(float4)) return EXL3_E_WORKSPACE;
     VerifyArgs a{};
     a.target = target; a.draft = draft;
     a.target_ld = target_ld; a.draft_ld = draft_ld; a.noise_ld = noise_ld;
     a.tokens = draft_tokens; a.cu_rows = cu_rows; a.temperature = temperature; a.u = u; a.noise = noise;
     a.out = tokens_out; a.count = count; a.prob = accept_prob;
+    a.stats = static_cast<float4*>(workspace);
     a.rows = rows; a.seqs = seqs; a.n = n; a.max_drafts = max_drafts;
+    a.chunks = p.chunks;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const dim3 grid(seqs), block(kVerifyThreads);
     switch (dtype) {
-    case EXL3_F16: return launch_pdl(verify_kernel<__half>, grid, block, 0, s, a);
-    case EXL3_BF16: return launch_pdl(verify_kernel<__nv_bfloat16>, grid, block, 0, s, a);
-    default: return launch_pdl(verify_kernel<float>, grid, block, 0, s, a);
+    case EXL3_F16: return launch_verify<__half>(a, p.per, s);
+    case EXL3_BF16: return launch_verify<__nv_bfloat16>(a, p.per, s);
+    default: return launch_verify<float>(a, p.per, s);
     }
 }

@@ -24,22 +24,24 @@ import math
 
 import torch
 
-from . import _lib
-from ._lib import PagedDesc, check, dtype_code, lib, stream_ptr
+from ._lib import PagedDesc, check, lib, stream_ptr
 
-_CACHE_DTYPES = (torch.float16, torch.bfloat16)
 _status: dict = {}
 _workspaces: dict = {}
 
 
-def _status_word(device: torch.device) -> torch.Tensor:
-    word = _status.get(device.index)
+_get_device = torch._C._cuda_getDevice
+_capturing = torch._C._cuda_isCurrentStreamCapturing
+
+
+def _status_word(index: int) -> int:
+    """Address of the device's status word."""
+    word = _status.get(index)
     if word is None:
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             raise RuntimeError("call a paged kernel once on this device before capturing it in a graph")
-        word = torch.zeros(4, dtype=torch.int32, device=device)
-        _status[device.index] = word
-    return word
+        word = _status[index] = torch.zeros(4, dtype=torch.int32, device=torch.device("cuda", index))
+    return word.data_ptr()
 
 
 def paged_status(device: torch.device | None = None) -> int:
@@ -62,41 +64,47 @@ def check_paged_status(device: torch.device | None = None) -> None:
                            "failed call are invalid")
 
 
-def _need(cond: bool, what: str) -> None:
-    if not cond:
-        raise ValueError(what)
+_F16, _BF16, _I32, _F32 = torch.float16, torch.bfloat16, torch.int32, torch.float32
 
 
-def _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows: int) -> PagedDesc:
-    """Checked descriptor of the batch: what can be checked without reading device memory."""
+def _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows: int) -> tuple[PagedDesc, int]:
+    """Checked descriptor of the batch (what can be checked without reading device memory) and its device."""
     dt = k_pages.dtype
-    if dt not in _CACHE_DTYPES or v_pages.dtype != dt:
+    if (dt is not _F16 and dt is not _BF16) or v_pages.dtype is not dt:
         raise TypeError("k_pages and v_pages must both be fp16 or both bf16")
-    if page_table.dtype != torch.int32 or cu_rows.dtype != torch.int32 or lens.dtype != torch.int32:
+    if page_table.dtype is not _I32 or cu_rows.dtype is not _I32 or lens.dtype is not _I32:
         raise TypeError("page_table, cu_rows and lens must be int32")
-    dev = k_pages.device
-    if dev.type != "cuda":
+    dev = k_pages.get_device()
+    if dev < 0:
         raise ValueError("EXL3 kernels take CUDA tensors")
-    _need(v_pages.device == dev and page_table.device == dev and cu_rows.device == dev and lens.device == dev,
-          "the pages and the batch's tables must be on one device")
+    if not (v_pages.get_device() == page_table.get_device() == cu_rows.get_device() == lens.get_device() == dev):
+        raise ValueError("the pages and the batch's tables must be on one device")
     shape = k_pages.shape
-    _need(len(shape) == 4 and v_pages.shape == shape, "pages must be (num_pages, hkv, page_size, head_dim), K and V alike")
-    _need(page_table.dim() == 2 and cu_rows.dim() == 1 and lens.dim() == 1, "page_table is 2-d, cu_rows and lens 1-d")
-    seqs, cols = page_table.shape
-    _need(seqs >= 1 and cu_rows.shape[0] == seqs + 1 and lens.shape[0] == seqs,
-          "page_table (seqs, cols), cu_rows (seqs + 1) and lens (seqs) must agree")
-    _need(k_pages.is_contiguous() and v_pages.is_contiguous(), "pages must be contiguous")
-    _need(page_table.is_contiguous() and cu_rows.is_contiguous() and lens.is_contiguous(),
-          "page_table, cu_rows and lens must be contiguous")
+    if len(shape) != 4 or v_pages.shape != shape:
+        raise ValueError("pages must be (num_pages, hkv, page_size, head_dim), K and V alike")
+    table = page_table.shape
+    if len(table) != 2 or cu_rows.dim() != 1 or lens.dim() != 1:
+        raise ValueError("page_table is 2-d, cu_rows and lens 1-d")
+    seqs, cols = table
+    if seqs < 1 or cu_rows.numel() != seqs + 1 or lens.numel() != seqs:
+        raise ValueError("page_table (seqs, cols), cu_rows (seqs + 1) and lens (seqs) must agree")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError("pages must be contiguous")
+    if not (page_table.is_contiguous() and cu_rows.is_contiguous() and lens.is_contiguous()):
+        raise ValueError("page_table, cu_rows and lens must be contiguous")
+    num, hkv, ps, hd = shape
     return PagedDesc(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), cu_rows.data_ptr(), lens.data_ptr(),
-                     seqs, rows, cols, shape[0], shape[2], shape[1], shape[3], 0 if dt is torch.float16 else 1)
+                     seqs, rows, cols, num, ps, hkv, hd, 0 if dt is _F16 else 1), dev
 
 
-def _strided(x: torch.Tensor, width: int, name: str) -> int:
+def _row_stride(x: torch.Tensor, width: int, name: str) -> int:
     """Row stride in elements of a (rows, width) view with contiguous rows."""
-    _need(x.dim() == 2 and x.shape[1] == width, f"{name} must be (rows, {width})")
-    _need(x.stride(1) == 1 and (x.shape[0] < 2 or x.stride(0) >= width), f"{name} needs contiguous, non-overlapping rows")
-    return max(x.stride(0), width)
+    if x.dim() != 2 or x.shape[1] != width:
+        raise ValueError(f"{name} must be (rows, {width})")
+    s0, s1 = x.stride()
+    if s1 != 1 or (s0 < width and x.shape[0] > 1):
+        raise ValueError(f"{name} needs contiguous, non-overlapping rows")
+    return s0 if s0 > width else width
 
 
 def paged_qkv_post(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm_w: torch.Tensor | None,
@@ -110,52 +118,70 @@ def paged_qkv_post(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm_w: 
     projection output are fine. cos / sin f32 (positions, rotated / 2): the first 2 * cos.shape[1] elements of a head
     are rotated. Computed in fp32 and rounded once, to the cache's dtype. Two live rows of a call must not share a position.
     """
-    rows = q.shape[0]
-    b = _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows)
-    hd, dt = b.head_dim, q.dtype
-    if dt not in _CACHE_DTYPES or k.dtype != dt or v.dtype != dt:
+    rows, width = q.shape
+    b, dev = _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows)
+    if _get_device() != dev:                      # the kernels launch on the current device
+        with torch.cuda.device(dev):
+            return paged_qkv_post(q, k, v, q_norm_w, k_norm_w, eps, cos, sin, k_pages, v_pages, page_table, cu_rows, lens, q_out)
+    hd, hkv, dt = b.head_dim, b.hkv, q.dtype
+    if (dt is not _F16 and dt is not _BF16) or k.dtype is not dt or v.dtype is not dt:
         raise TypeError("q, k and v must all be fp16 or all bf16")
-    _need(k.shape[0] == rows and v.shape[0] == rows, "q, k and v must have the same rows")
-    _need(q.dim() == 2 and q.shape[1] > 0 and q.shape[1] % (b.hkv * hd) == 0,
-          "q's width must be a multiple of hkv * head_dim")
-    hq = q.shape[1] // hd
-    sq, sk, sv = _strided(q, hq * hd, "q"), _strided(k, b.hkv * hd, "k"), _strided(v, b.hkv * hd, "v")
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    if k.shape[0] != rows or v.shape[0] != rows:
+        raise ValueError("q, k and v must have the same rows")
+    if width == 0 or width % (hkv * hd):
+        raise ValueError("q's width must be a multiple of hkv * head_dim")
+    hq = width // hd
+    sq, sk, sv = _row_stride(q, width, "q"), _row_stride(k, hkv * hd, "k"), _row_stride(v, hkv * hd, "v")
+    if cos.dtype is not _F32 or sin.dtype is not _F32:
         raise TypeError("cos and sin must be fp32")
-    _need(cos.dim() == 2 and cos.shape == sin.shape and cos.is_contiguous() and sin.is_contiguous(),
-          "cos and sin must be contiguous (positions, rotated / 2)")
-    dev = k_pages.device
-    _need(q.device == dev and k.device == dev and v.device == dev and cos.device == dev and sin.device == dev,
-          "all tensors must be on one device")
-    for w in (q_norm_w, k_norm_w):
+    if cos.dim() != 2 or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError("cos and sin must be contiguous (positions, rotated / 2)")
+    if not (q.get_device() == k.get_device() == v.get_device() == cos.get_device() == sin.get_device() == dev):
+        raise ValueError("all tensors must be on one device")
+    weights = [None, None]
+    for i, w in enumerate((q_norm_w, k_norm_w)):
         if w is not None:
-            if w.dtype != dt:
+            if w.dtype is not dt:
                 raise TypeError("norm weights must have q's dtype")
-            _need(w.numel() == hd and w.is_contiguous() and w.device == dev, "norm weights must be contiguous (head_dim)")
+            if w.numel() != hd or not w.is_contiguous() or w.get_device() != dev:
+                raise ValueError("norm weights must be contiguous (head_dim) on the pages' device")
+            weights[i] = w.data_ptr()
     if q_out is None:
-        q_out = torch.empty((rows, hq, hd), dtype=k_pages.dtype, device=dev)
-    else:
-        _need(q_out.shape == (rows, hq, hd) and q_out.dtype == k_pages.dtype and q_out.is_contiguous()
-              and q_out.device == dev, "q_out must be contiguous (rows, hq, head_dim) in the cache's dtype")
-    with torch.cuda.device(dev):
-        check(lib().exl3_paged_qkv_post(b, q.data_ptr(), k.data_ptr(), v.data_ptr(), sq, sk, sv,
-                                        0 if dt is torch.float16 else 1, hq,
-                                        None if q_norm_w is None else q_norm_w.data_ptr(),
-                                        None if k_norm_w is None else k_norm_w.data_ptr(), eps, cos.data_ptr(),
-                                        sin.data_ptr(), cos.shape[0], cos.shape[1], q_out.data_ptr(),
-                                        _status_word(dev).data_ptr(), stream_ptr(dev)), "exl3_paged_qkv_post")
+        q_out = torch.empty((rows, hq, hd), dtype=k_pages.dtype, device=k_pages.device)
+    elif (q_out.shape != (rows, hq, hd) or q_out.dtype is not k_pages.dtype or not q_out.is_contiguous()
+          or q_out.get_device() != dev):
+        raise ValueError("q_out must be contiguous (rows, hq, head_dim) in the cache's dtype")
+    n_rope, half = cos.shape
+    status = lib().exl3_paged_qkv_post(b, q.data_ptr(), k.data_ptr(), v.data_ptr(), sq, sk, sv, 0 if dt is _F16 else 1, hq,
+                                       weights[0], weights[1], eps, cos.data_ptr(), sin.data_ptr(), n_rope, half,
+                                       q_out.data_ptr(), _status_word(dev), stream_ptr(dev))
+    if status:
+        check(status, "exl3_paged_qkv_post")
     return q_out
 
 
-def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+def _workspace(index: int, stream: int, nbytes: int) -> torch.Tensor:
     """Scratch of this device and stream: calls on different streams may overlap, calls on one stream run one after
     another. A captured call gets scratch of its own from the graph's pool: replays may run beside eager calls."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    ws = _workspaces.get((device.index, stream))
+    if _capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+    ws = _workspaces.get((index, stream))
     if ws is None or ws.numel() < nbytes:
-        ws = _workspaces[(device.index, stream)] = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws = _workspaces[(index, stream)] = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
     return ws
+
+
+_attn_bytes: dict = {}
+
+
+def _attn_workspace_bytes(b: PagedDesc, hq: int, dev: int) -> int:
+    """Depends on the device and the head size alone."""
+    need = _attn_bytes.get((dev, b.head_dim))
+    if need is None:
+        size = ctypes.c_size_t()
+        check(lib().exl3_paged_attn_workspace(b, hq, ctypes.byref(size)), "exl3_paged_attn_workspace")
+        need = _attn_bytes[(dev, b.head_dim)] = size.value
+    return need
 
 
 def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -166,33 +192,39 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     (rows, hq, head_dim) in q's dtype, which is the cache's. Rows at negative positions give zeros; what lies behind a
     sequence's end in its pages is never used.
     """
-    rows = q.shape[0]
-    b = _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows)
-    dev = k_pages.device
-    if q.dtype != k_pages.dtype:
+    if q.dim() != 3:
+        raise ValueError("q must be (rows, hq, head_dim)")
+    rows, hq, hd = q.shape
+    b, dev = _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows)
+    if _get_device() != dev:                      # the kernels launch on the current device
+        with torch.cuda.device(dev):
+            return paged_attn(q, k_pages, v_pages, page_table, cu_rows, lens, scale, out)
+    if q.dtype is not k_pages.dtype:
         raise TypeError("q must have the cache's dtype")
-    _need(q.dim() == 3 and q.shape[2] == b.head_dim and q.device == dev, "q must be (rows, hq, head_dim) on the pages' device")
-    hq, hd = q.shape[1], b.head_dim
-    _need(hq >= 1 and hq % b.hkv == 0 and hq // b.hkv <= 128, "hq must be a multiple of hkv, at most 128 heads per kv head")
+    if hd != b.head_dim or q.get_device() != dev:
+        raise ValueError("q must be (rows, hq, head_dim) on the pages' device")
+    if hq < 1 or hq % b.hkv or hq // b.hkv > 128:
+        raise ValueError("hq must be a multiple of hkv, at most 128 heads per kv head")
     if scale is None:
         scale = 1.0 / math.sqrt(hd)
-    _need(scale > 0 and math.isfinite(scale), "scale must be positive")
-    if q.stride(2) != 1 or q.stride(1) != hd or q.stride(0) % 8 or q.stride(0) < hq * hd or q.data_ptr() % 16:
+    elif not (scale > 0 and math.isfinite(scale)):
+        raise ValueError("scale must be positive")
+    s0, s1, s2 = q.stride()
+    if s2 != 1 or s1 != hd or s0 % 8 or s0 < hq * hd or q.data_ptr() % 16:
         q = q.contiguous()
+        s0 = hq * hd
     if out is None:
-        out = torch.empty((rows, hq, hd), dtype=q.dtype, device=dev)
-    else:
-        _need(out.shape == (rows, hq, hd) and out.dtype == q.dtype and out.is_contiguous() and out.device == dev,
-              "out must be contiguous (rows, hq, head_dim) in q's dtype")
+        out = torch.empty((rows, hq, hd), dtype=q.dtype, device=q.device)
+    elif out.shape != (rows, hq, hd) or out.dtype is not q.dtype or not out.is_contiguous() or out.get_device() != dev:
+        raise ValueError("out must be contiguous (rows, hq, head_dim) in q's dtype")
     if rows == 0:
         return out
-    with torch.cuda.device(dev):
-        stream = stream_ptr(dev)
-        need = ctypes.c_size_t()
-        check(lib().exl3_paged_attn_workspace(b, hq, ctypes.byref(need)), "exl3_paged_attn_workspace")
-        ws = _workspace(dev, stream, need.value)
-        check(lib().exl3_paged_attn(b, q.data_ptr(), q.stride(0), hq, scale, out.data_ptr(), ws.data_ptr(), ws.numel(),
-                                    _status_word(dev).data_ptr(), stream), "exl3_paged_attn")
+    stream = stream_ptr(dev)
+    ws = _workspace(dev, stream, _attn_workspace_bytes(b, hq, dev))
+    status = lib().exl3_paged_attn(b, q.data_ptr(), s0, hq, scale, out.data_ptr(), ws.data_ptr(), ws.numel(),
+                                   _status_word(dev), stream)
+    if status:
+        check(status, "exl3_paged_attn")
     return out
 
 

@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from ._lib import check, dtype_code, lib, stream_ptr
-from .paged import _need, _workspace
+from .paged import _F32, _I32, _get_device, _row_stride, _workspace
 
 
 def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, cu_rows: torch.Tensor, u: torch.Tensor,
@@ -31,47 +31,59 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, cu_ro
     """
     dt = target_logits.dtype
     code = dtype_code(dt)
-    dev = target_logits.device
-    if dev.type != "cuda":
+    dev = target_logits.get_device()
+    if dev < 0:
         raise ValueError("EXL3 kernels take CUDA tensors")
-    _need(target_logits.dim() == 2 and cu_rows.dim() == 1 and cu_rows.shape[0] >= 2, "target_logits (rows, n), cu_rows (seqs + 1)")
+    if _get_device() != dev:                      # the kernels launch on the current device
+        with torch.cuda.device(dev):
+            return verify_drafts(target_logits, draft_tokens, cu_rows, u, noise, max_drafts, draft_logits, temperature)
+    if target_logits.dim() != 2 or cu_rows.dim() != 1 or cu_rows.numel() < 2:
+        raise ValueError("need target_logits (rows, n) and cu_rows (seqs + 1)")
     rows, n = target_logits.shape
-    seqs = cu_rows.shape[0] - 1
+    seqs = cu_rows.numel() - 1
     drafts = rows - seqs
-    _need(n >= 1 and drafts >= 0 and max_drafts >= 0, "each sequence needs at least one target row")
-    if cu_rows.dtype != torch.int32 or draft_tokens.dtype != torch.int64:
+    if n < 1 or drafts < 0 or max_drafts < 0:
+        raise ValueError("each sequence needs at least one target row")
+    if cu_rows.dtype is not _I32 or draft_tokens.dtype is not torch.int64:
         raise TypeError("cu_rows must be int32 and draft_tokens int64")
-    if u.dtype != torch.float32 or noise.dtype != torch.float32 or (temperature is not None and temperature.dtype != torch.float32):
+    if u.dtype is not _F32 or noise.dtype is not _F32 or (temperature is not None and temperature.dtype is not _F32):
         raise TypeError("u, noise and temperature must be fp32")
-    _need(draft_tokens.shape == (drafts,) and u.shape == (drafts,), "draft_tokens and u must be (rows - seqs)")
-    _need(noise.shape == (seqs, n) and (temperature is None or temperature.shape == (seqs,)),
-          "noise must be (seqs, n) and temperature (seqs)")
-    _need(cu_rows.is_contiguous() and draft_tokens.is_contiguous() and u.is_contiguous()
-          and (temperature is None or temperature.is_contiguous()), "cu_rows, draft_tokens, u and temperature must be contiguous")
-    matrices = [target_logits, noise]
+    if draft_tokens.shape != (drafts,) or u.shape != (drafts,):
+        raise ValueError("draft_tokens and u must be (rows - seqs)")
+    if noise.shape != (seqs, n) or (temperature is not None and temperature.shape != (seqs,)):
+        raise ValueError("noise must be (seqs, n) and temperature (seqs)")
+    if not (cu_rows.is_contiguous() and draft_tokens.is_contiguous() and u.is_contiguous()
+            and (temperature is None or temperature.is_contiguous())):
+        raise ValueError("cu_rows, draft_tokens, u and temperature must be contiguous")
+    if not (draft_tokens.get_device() == cu_rows.get_device() == u.get_device() == noise.get_device() == dev):
+        raise ValueError("all tensors must be on one device")
+    ld, noise_ld = _row_stride(target_logits, n, "target_logits"), _row_stride(noise, n, "noise")
+    draft_ptr, draft_ld, temp_ptr = None, n, None
     if draft_logits is not None:
-        if draft_logits.dtype != dt:
+        if draft_logits.dtype is not dt:
             raise TypeError("draft_logits must have target_logits' dtype")
-        _need(draft_logits.shape == (drafts, n), "draft_logits must be (rows - seqs, n)")
-        matrices.append(draft_logits)
-    for m in matrices:
-        _need(m.stride(1) == 1 and (m.shape[0] < 2 or m.stride(0) >= n), "logits and noise need contiguous, non-overlapping rows")
-    for t in (draft_tokens, cu_rows, u, noise, draft_logits, temperature):
-        _need(t is None or t.device == dev, "all tensors must be on one device")
-    tokens = torch.empty((seqs, max_drafts + 1), dtype=torch.int64, device=dev)
-    count = torch.empty(seqs, dtype=torch.int32, device=dev)
-    prob = torch.empty(drafts, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        stream = stream_ptr(dev)
-        need = ctypes.c_size_t()
-        check(lib().exl3_verify_workspace(rows, seqs, n, ctypes.byref(need)), "exl3_verify_workspace")
-        ws = _workspace(dev, stream, need.value)
-        check(lib().exl3_verify_drafts(target_logits.data_ptr(), max(target_logits.stride(0), n),
-                                       None if draft_logits is None or drafts == 0 else draft_logits.data_ptr(),
-                                       n if draft_logits is None else max(draft_logits.stride(0), n), code, rows, seqs, n,
-                                       draft_tokens.data_ptr() if drafts else None, cu_rows.data_ptr(),
-                                       None if temperature is None else temperature.data_ptr(),
-                                       u.data_ptr() if drafts else None, noise.data_ptr(), max(noise.stride(0), n),
-                                       max_drafts, tokens.data_ptr(), count.data_ptr(), prob.data_ptr() if drafts else None,
-                                       ws.data_ptr(), ws.numel(), stream), "exl3_verify_drafts")
+        if draft_logits.shape != (drafts, n) or draft_logits.get_device() != dev:
+            raise ValueError("draft_logits must be (rows - seqs, n) on target_logits' device")
+        draft_ld = _row_stride(draft_logits, n, "draft_logits")
+        if drafts:
+            draft_ptr = draft_logits.data_ptr()
+    if temperature is not None:
+        if temperature.get_device() != dev:
+            raise ValueError("all tensors must be on one device")
+        temp_ptr = temperature.data_ptr()
+    device = target_logits.device
+    tokens = torch.empty((seqs, max_drafts + 1), dtype=torch.int64, device=device)
+    count = torch.empty(seqs, dtype=_I32, device=device)
+    prob = torch.empty(drafts, dtype=_F32, device=device)
+    stream = stream_ptr(dev)
+    size = ctypes.c_size_t()
+    check(lib().exl3_verify_workspace(rows, seqs, n, size), "exl3_verify_workspace")
+    ws = _workspace(dev, stream, size.value)
+    status = lib().exl3_verify_drafts(target_logits.data_ptr(), ld, draft_ptr, draft_ld, code, rows, seqs, n,
+                                      draft_tokens.data_ptr() if drafts else None, cu_rows.data_ptr(), temp_ptr,
+                                      u.data_ptr() if drafts else None, noise.data_ptr(), noise_ld, max_drafts,
+                                      tokens.data_ptr(), count.data_ptr(), prob.data_ptr() if drafts else None, ws.data_ptr(),
+                                      ws.numel(), stream)
+    if status:
+        check(status, "exl3_verify_drafts")
     return tokens, count, prob
