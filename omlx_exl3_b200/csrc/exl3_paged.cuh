@@ -13,15 +13,17 @@ namespace exl3 {
 // page table's columns or the rotation table): the row or page is left out and this bit is set.
 enum : uint32_t { kStatusPagedRange = 8u };
 
-// The sequence of `row`: the first s with row < cu_rows[s + 1], found by the whole warp with 32 probes a
-// round (one round up to 32 sequences, two up to 1024). seqs >= 1 and row < cu_rows[seqs].
-__device__ __forceinline__ int seq_of_row(const int32_t* cu_rows, int seqs, int row, int lane)
+// The first s with x < cu_rows[s + 1] - skip * (s + 1), found by the whole warp with 32 probes a round (one round up to
+// 32 sequences, two up to 1024). skip 0: the sequence of row x; skip 1: that of draft x, where every sequence has a draft for each
+// row but its last. seqs >= 1; x at or past the end gives the last sequence.
+template <int skip = 0>
+__device__ __forceinline__ int seq_of_row(const int32_t* cu_rows, int seqs, int x, int lane)
 {
     int lo = 0, n = seqs;                                // the answer is in [lo, lo + n)
     while (n > 1) {
         const int step = (n + 31) >> 5;                  // probe the last sequence of each of 32 parts
         const int probe = min(lo + (lane + 1) * step, lo + n);
-        const unsigned past = __ballot_sync(0xffffffffu, cu_rows[probe] <= row);
+        const unsigned past = __ballot_sync(0xffffffffu, cu_rows[probe] - skip * probe <= x);
         const int part = min(__popc(past), 31);
         const int end = lo + n;
         lo = min(lo + part * step, end - 1);

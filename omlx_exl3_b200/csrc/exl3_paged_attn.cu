@@ -105,6 +105,78 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16])
         : "memory");
 }
 
+// Two fp32 values in one 64-bit register: the packed fp32 instructions do both in one issue slot.
+__device__ __forceinline__ uint64_t f2(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void f2_get(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// Largest of three.
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// One lane of the (converged) warp: 1 in it, 0 in the others.
+__device__ __forceinline__ uint32_t elect_one()
+{
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r;
+}
+
+// A value that is the same in all lanes, known to the compiler as such.
+__device__ __forceinline__ uint64_t uniform64(uint64_t x)
+{
+    const uint32_t lo = __shfl_sync(0xffffffffu, (uint32_t)x, 0), hi = __shfl_sync(0xffffffffu, (uint32_t)(x >> 32), 0);
+    return ((uint64_t)hi << 32) | lo;
+}
+
+// tcgen05.mma / commit issued by the lanes with go != 0 (one of the warp).
+__device__ __forceinline__ void tc_mma_if(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t go)
+{
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(go)
+        : "memory");
+}
+
+__device__ __forceinline__ void tc_mma_ts_if(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t go)
+{
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(go)
+        : "memory");
+}
+
+__device__ __forceinline__ void tc_commit_if(uint64_t* bar, uint32_t go)
+{
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_addr(bar)),
+        "r"(go)
+        : "memory");
+}
+
 // Bounded wait of a whole warp, with one answer for all its lanes.
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, uint64_t limit_ns = 2000000000ull)
 {
@@ -129,22 +201,29 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     uint64_t* q_full = empty + P::kStages;
     uint64_t* q_empty = q_full + 1;                   // the item's S are done and its merge buffer is read
     uint64_t* s_full = q_empty + 1;                   // [2] S of the slot is complete (and the P V before it)
-    uint64_t* p_full = s_full + 2;                    // [2] P of the slot is written
-    uint64_t* o_full = p_full + 2;                    // [2] the slot's accumulator is complete
+    uint64_t* p_full = s_full + 2;                    // [2][2] half of P of the slot is written
+    uint64_t* v_dirty = p_full + 4;                   // the item's last V tile has landed and reaches past the sequence's end
+    uint64_t* v_clean = v_dirty + 1;                  // it is zero there
+    uint64_t* turn = v_clean + 1;                     // [2] the slot's MMAs of a step may be issued
+    uint64_t* o_full = turn + 2;                   // [2] the slot's accumulator is complete
     uint64_t* o_empty = o_full + 2;                   // [2] it has been read
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < P::kStages; ++i) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+            mbar_init(&empty[i], 2);
         }
         mbar_init(q_full, 1);
-        mbar_init(q_empty, 1 + 8);
+        mbar_init(q_empty, 2 + 8);
+        mbar_init(v_dirty, 1);
+        mbar_init(v_clean, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[2 * i], 4);
+            mbar_init(&p_full[2 * i + 1], 4);
+            mbar_init(&turn[i], 1);
             mbar_init(&o_full[i], 1);
             mbar_init(&o_empty[i], 4);
         }
@@ -242,116 +321,138 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         for (uint32_t i = it > (uint32_t)P::kStages ? it - P::kStages : 0; i < it; ++i)
             if (!pa_wait(&full[i % P::kStages], (i / P::kStages) & 1, kPaExitNs)) ok = false;
         if (n_seg > 0 && !pa_wait(q_full, (n_seg - 1) & 1, kPaExitNs)) ok = false;
-      } else if (warp == 9) {
+      } else if (warp == 10) {
         sched.start(blockIdx.x, gridDim.x, lane);
-        // ---------------------------------------------------------------- MMAs (lane 0 issues)
-        constexpr uint32_t idesc_s = pa_idesc<C>(kPaStep, false), idesc_o = pa_idesc<C>(HD, true);
-        uint32_t n_seg = 0, it = 0, n_p[2] = {0, 0}, n_o[2] = {0, 0};
-        auto stage_wait = [&](uint32_t i) {
-            if (ok && !pa_wait(&full[i % P::kStages], (i / P::kStages) & 1)) ok = false;
-            tc_fence_after();
-            return kv_s + (i % P::kStages) * P::kTile;
-        };
-        auto mma_s = [&](int slot, int tile, const uint8_t* k) {
-            if (!ok || lane != 0) return;
-            const uint64_t qd = smem_desc_sw128(q_s + tile * P::kTile), kd = smem_desc_sw128(k);
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk) {
-                const int off = ((kk / 4) * P::kPanel + (kk % 4) * 32) >> 4;
-                tc_mma_f16(tmem + slot * kPaStep, qd + off, kd + off, idesc_s, kk > 0);
-            }
-            tc_commit(&s_full[slot]);
-        };
-        auto mma_o = [&](int slot, const uint8_t* v, bool first) {
-            if (ok && !pa_wait(&p_full[slot], n_p[slot] & 1)) ok = false;
-            ++n_p[slot];
-            if (first) {
-                if (n_o[slot] > 0 && ok && !pa_wait(&o_empty[slot], (n_o[slot] - 1) & 1)) ok = false;
-                ++n_o[slot];
-            }
-            tc_fence_after();
-            if (!ok || lane != 0) return;
-            const uint64_t vd = pa_desc_v(v, P::kPanel);
-#pragma unroll
-            for (int kk = 0; kk < kPaStep / 16; ++kk)
-                tc_mma_f16_ts(tmem + 256 + slot * HD, tmem + slot * kPaStep + kk * 8, vd + kk * (2048 >> 4), idesc_o,
-                              (first && kk == 0) ? 0u : 1u);
-        };
-        auto commit = [&](uint64_t* bar) {
-            if (ok && lane == 0) tc_commit(bar);
-        };
-        // positions past the sequence's end: their V rows become zero
-        auto clean = [&](uint8_t* v, int step) {
-            const int valid = g.end - step * kPaStep;
-            if (valid >= kPaStep) return;
-            const int lo = max(valid, 0) * 8;
-            for (int i = lo + lane; i < kPaStep * 8; i += 32)
+        // ---------------------------------------------------------------- V behind the sequence's end becomes zero
+        uint32_t it = 0, n = 0;
+        while (ok && sched.next(g)) {
+            it += 2 * (g.j1 - g.j0);                                   // the segment's last tile is its last V
+            const int valid = g.end - (g.j1 - 1) * kPaStep;
+            if (valid >= kPaStep) continue;
+            if (!pa_wait(v_dirty, n++ & 1)) { ok = false; break; }
+            uint8_t* v = kv_s + ((it - 1) % P::kStages) * P::kTile;
+            for (int i = max(valid, 0) * 8 + lane; i < kPaStep * 8; i += 32)
 #pragma unroll
                 for (int p = 0; p < P::kPanels; ++p)
                     *reinterpret_cast<uint4*>(v + p * P::kPanel + i * 16) = make_uint4(0, 0, 0, 0);
             fence_proxy_async_smem();
             __syncwarp();
+            if (lane == 0) mbar_arrive(v_clean);
+        }
+      } else {
+        sched.start(blockIdx.x, gridDim.x, lane);
+        // ---------------------------------------------------------------- MMAs: warp 9 for slot 0, warp 11 for slot 1
+        // Between the MMAs of a step lie waits and commits of some hundred cycles in the issuing warp; with a warp per slot
+        // they pass while the other slot's MMAs run. Each whole warp runs this and one elected lane issues, so that operands
+        // come from uniform registers. Both warps see every tile of the ring land and release it (the tiles of the other
+        // slot at once), so neither can fall a round behind.
+        constexpr uint32_t idesc_s = pa_idesc<C>(kPaStep, false), idesc_o = pa_idesc<C>(HD, true);
+        const int slot = warp == 11;
+        const uint32_t leader = elect_one();
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint32_t s_tm = tm + slot * kPaStep, o_tm = tm + 256 + slot * HD;
+        const uint64_t q_desc = uniform64(smem_desc_sw128(q_s)), k_desc = uniform64(smem_desc_sw128(kv_s)),
+                       v_desc = uniform64(pa_desc_v(kv_s, P::kPanel));
+        uint32_t n_seg = 0, n_clean = 0, st = 0, ring = 0, n_p = 0, n_o = 0;   // st: stage of the ring, ring: its round
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            if (ok && !pa_wait(bar, parity)) ok = false;
+        };
+        auto commit = [&](uint64_t* bar) { tc_commit_if(bar, leader & (uint32_t)ok); };
+        auto take = [&]() {                                            // the stage of the ring's next tile, once it has landed
+            const uint32_t i = st;
+            wait(&full[i], ring & 1);
+            if (++st == (uint32_t)P::kStages) {
+                st = 0;
+                ++ring;
+            }
+            return i;
+        };
+        auto release = [&](uint32_t i, bool mine) {
+            if (mine) commit(&empty[i]);
+            else if (ok && lane == 0) mbar_arrive(&empty[i]);
+        };
+        auto mma_s = [&](int tile, uint32_t stage) {
+            const uint64_t qd = q_desc + tile * (P::kTile >> 4), kd = k_desc + stage * (P::kTile >> 4);
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+                const int off = ((kk / 4) * P::kPanel + (kk % 4) * 32) >> 4;
+                tc_mma_if(s_tm, qd + off, kd + off, idesc_s, kk > 0, leader & (uint32_t)ok);
+            }
+            commit(&s_full[slot]);
+        };
+        // Turns: the slots issue their steps' MMAs alternately. Left alone the two fall into step, both in softmax and then both
+        // at the tensor core (602 against 507 us for the 4096-row chunk over 8192 positions).
+        uint32_t n_turn = 0;
+        auto my_turn = [&]() {
+            if (slot == 1 || n_turn > 0) wait(&turn[slot], (n_turn - (slot == 0 ? 1 : 0)) & 1);
+            ++n_turn;
+        };
+        auto pass_turn = [&]() {
+            if (ok && lane == 0) mbar_arrive(&turn[slot ^ 1]);
+        };
+        // P V of a step; `first`: the slot's first of the item
+        auto mma_o = [&](uint32_t stage, bool first) {
+            if (first) {
+                if (n_o > 0) wait(&o_empty[slot], (n_o - 1) & 1);
+                ++n_o;
+            }
+            const uint64_t vd = v_desc + stage * (P::kTile >> 4);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                wait(&p_full[2 * slot + half], n_p & 1);
+                if (half == 0) my_turn();
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                    tc_mma_ts_if(o_tm, s_tm + kk * 8, vd + kk * (2048 >> 4), idesc_o, (first && kk == 0) ? 0u : 1u,
+                                 leader & (uint32_t)ok);
+            }
+            ++n_p;
         };
         while (ok && sched.next(g)) {
-            if (!pa_wait(q_full, n_seg & 1)) { ok = false; break; }
+            wait(q_full, n_seg & 1);
             ++n_seg;
-            const int n = g.j1 - g.j0;
-            if (item_of(g).dual) {
-                const uint8_t* k = stage_wait(it);
-                mma_s(0, 0, k);
-                mma_s(1, 1, k);
-                commit(&empty[it % P::kStages]);
-                ++it;
-                if (n == 1) commit(q_empty);
-                for (int m = 0; m < n && ok; ++m) {
-                    const uint32_t vi = it, ki = it + 1;
-                    uint8_t* v = stage_wait(vi);
-                    clean(v, g.j0 + m);
-                    const bool more = m + 1 < n;
-                    mma_o(0, v, m == 0);
-                    if (more) {
-                        k = stage_wait(ki);
-                        mma_s(0, 0, k);
-                    } else {
-                        commit(&o_full[0]);
-                    }
-                    mma_o(1, v, m == 0);
-                    commit(&empty[vi % P::kStages]);
-                    if (more) {
-                        mma_s(1, 1, k);
-                        commit(&empty[ki % P::kStages]);
-                        if (m + 2 == n) commit(q_empty);
-                    } else {
-                        commit(&o_full[1]);
-                    }
-                    it += more ? 2 : 1;
+            const int n = __shfl_sync(0xffffffffu, g.j1 - g.j0, 0);
+            const bool dirty = __shfl_sync(0xffffffffu, g.j1 * kPaStep > g.end, 0);   // the last V tile reaches past the end
+            const bool dual = __shfl_sync(0xffffffffu, item_of(g).dual, 0);
+            const int ahead = dual ? 1 : 2;                            // K tiles before the first V
+            for (int i = 0; i < min(n, ahead); ++i) {
+                const uint32_t k = take();
+                const bool mine = dual || i == slot;
+                if (mine) {
+                    tc_fence_after();
+                    mma_s(dual ? slot : 0, k);
                 }
-            } else {
-                for (int i = 0; i < min(n, 2); ++i, ++it) {
-                    mma_s(i, 0, stage_wait(it));
-                    commit(&empty[it % P::kStages]);
+                release(k, mine);
+            }
+            if (n <= ahead) commit(q_empty);
+            for (int m = 0; m < n; ++m) {
+                const bool mine = dual || (m & 1) == slot, more = m + ahead < n;
+                const uint32_t v = take();
+                uint32_t k = 0;
+                if (more) k = take();
+                if (m + 1 == n && dirty) {                             // warp 10 cleans it, once per such item
+                    if (lane == 0 && (dual ? slot == 0 : mine)) mbar_arrive(v_dirty);
+                    wait(v_clean, n_clean++ & 1);
                 }
-                if (n <= 2) commit(q_empty);
-                for (int m = 0; m < n && ok; ++m) {
-                    const int slot = m & 1;
-                    uint8_t* v = stage_wait(it);
-                    clean(v, g.j0 + m);
-                    mma_o(slot, v, m < 2);
-                    commit(&empty[it % P::kStages]);
-                    ++it;
-                    if (m + 2 < n) {
-                        mma_s(slot, 0, stage_wait(it));
-                        commit(&empty[it % P::kStages]);
-                        ++it;
-                        if (m + 3 == n) commit(q_empty);
-                    } else {
-                        commit(&o_full[slot]);
-                    }
+                if (mine) {
+                    mma_o(v, m < ahead);
+                    if (more) mma_s(dual ? slot : 0, k);
+                    else commit(&o_full[slot]);
+                    pass_turn();
                 }
+                release(v, mine);
+                if (more) release(k, mine);
+                if (m + 1 + ahead == n) commit(q_empty);
+            }
+            if (!dual && n % 2 && slot == 1) {
+                my_turn();
+                pass_turn();
             }
         }
         // the MMAs' last reads and commits before the CTA's memory goes
-        for (uint32_t i = it > (uint32_t)P::kStages ? it - P::kStages : 0; i < it; ++i)
+        const uint32_t taken = ring * P::kStages + st;
+        for (uint32_t i = taken > (uint32_t)P::kStages ? taken - P::kStages : 0; i < taken; ++i)
             if (!pa_wait(&empty[i % P::kStages], (i / P::kStages) & 1, kPaExitNs)) ok = false;
       }
     } else {
@@ -372,7 +473,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
             const int used = im.ntok[tile] * a.grp;
             const int tok = r / a.grp;
             const int pos = im.pos0 + tile * tokens + tok;
-            const int limit = r < used ? min(pos + 1, g.end) : 0;      // positions this row sees
+            const int limit = r < used ? min(pos + 1, g.end) : 0x7fffffff;    // positions this row sees; unused rows: any
             const bool idle = quarter * 32 >= used;                    // no row of this warp is used
             float m = -INFINITY, l = 0.f;
             const int n = g.j1 - g.j0;
@@ -392,15 +493,18 @@ __global__ void __launch_bounds__(kPaThreads, 1)
 #pragma unroll
                         for (int q = 0; q < kPaStep; ++q) x[q] = q < see ? x[q] : -INFINITY;
                     }
-                    float t0 = x[0], t1 = x[1], t2 = x[2], t3 = x[3];
+                    float t0 = max3(x[0], x[1], x[2]), t1 = max3(x[3], x[4], x[5]);
+                    float t2 = max3(x[6], x[7], x[8]), t3 = max3(x[9], x[10], x[11]);
 #pragma unroll
-                    for (int q = 4; q < kPaStep; q += 4) {
-                        t0 = fmaxf(t0, x[q]);
-                        t1 = fmaxf(t1, x[q + 1]);
-                        t2 = fmaxf(t2, x[q + 2]);
-                        t3 = fmaxf(t3, x[q + 3]);
+                    for (int q = 12; q + 8 <= kPaStep; q += 8) {
+                        t0 = max3(t0, x[q], x[q + 1]);
+                        t1 = max3(t1, x[q + 2], x[q + 3]);
+                        t2 = max3(t2, x[q + 4], x[q + 5]);
+                        t3 = max3(t3, x[q + 6], x[q + 7]);
                     }
-                    const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+                    t0 = max3(t0, x[kPaStep - 4], x[kPaStep - 3]);
+                    t1 = max3(t1, x[kPaStep - 2], x[kPaStep - 1]);
+                    const float top = max3(max3(t0, t1, t2), t3, t3);
                     const bool grow = (top - m) * c > kPaSlack;        // false for a row that has seen nothing yet
                     if (__any_sync(0xffffffffu, grow)) {
                         const float f = grow ? pa_weight(m, top, c) : 1.f;
@@ -421,30 +525,47 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                         }
                     }
                     const float mc = m == -INFINITY ? 0.f : m * c;
-                    float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
+                    const uint64_t c2 = f2(c, c), mc2 = f2(-mc, -mc);
+                    uint64_t l01 = f2(0.f, 0.f), l23 = l01;
+                    // p of the row, stored by 32 columns; the first half's P V runs beside the second half's exp
 #pragma unroll
                     for (int part = 0; part < 4; ++part) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int q = 0; q < 32; q += 4) {
                             const float* y = x + part * 32 + q;
-                            const float e0 = ex2(fmaf(y[0], c, -mc)), e1 = ex2(fmaf(y[1], c, -mc));
-                            const float e2 = ex2(fmaf(y[2], c, -mc)), e3 = ex2(fmaf(y[3], c, -mc));
-                            l0 += e0;
-                            l1 += e1;
-                            l2 += e2;
-                            l3 += e3;
+                            float e0, e1, e2, e3;
+                            f2_get(f2_fma(f2(y[0], y[1]), c2, mc2), e0, e1);
+                            f2_get(f2_fma(f2(y[2], y[3]), c2, mc2), e2, e3);
+                            e0 = ex2(e0);
+                            e1 = ex2(e1);
+                            e2 = ex2(e2);
+                            e3 = ex2(e3);
+                            l01 = f2_add(l01, f2(e0, e1));
+                            l23 = f2_add(l23, f2(e2, e3));
                             pk[q / 2] = pack2<C>(e0, e1);
                             pk[q / 2 + 1] = pack2<C>(e2, e3);
                         }
                         tc_st16(s_t + part * 16, pk);
+                        if (part == 1) {
+                            tc_wait_st();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&p_full[2 * slot]);
+                        }
                     }
+                    float l0, l1, l2, l3;
+                    f2_get(l01, l0, l1);
+                    f2_get(l23, l2, l3);
                     l += (l0 + l1) + (l2 + l3);
                     tc_wait_st();
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[slot]);
+                if (lane == 0) {
+                    if (idle) mbar_arrive(&p_full[2 * slot]);
+                    mbar_arrive(&p_full[2 * slot + 1]);
+                }
             }
             if (mine > 0) {
                 if (ok && !pa_wait(&o_full[slot], n_o & 1)) ok = false;

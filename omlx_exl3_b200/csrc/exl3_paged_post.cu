@@ -4,6 +4,8 @@
 //   xn = x * rsqrt(mean(x^2) + eps) * w ;  (a, b) = (xn[c], xn[c + R]) -> (a cos - b sin, b cos + a sin), c < R
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "exl3_b200.h"
 #include "exl3_common.cuh"
 #include "exl3_host.h"
@@ -19,113 +21,149 @@ struct PagedPostArgs {
     void* q_out;
     uint32_t* status;
     float eps;
-    int hq, rope_rows, rope_half, vec;
+    int hq, rope_rows, rope_half;
+    int per_row;                                     // warps of a row
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8])
+// Four consecutive elements as they are stored; VEC: one 8-byte load.
+template <typename T, bool VEC>
+__device__ __forceinline__ uint2 load4(const T* p)
 {
-    if (vec) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        const T* e = reinterpret_cast<const T*>(&u);
+    if constexpr (VEC) return *reinterpret_cast<const uint2*>(p);
+    const unsigned short* e = reinterpret_cast<const unsigned short*>(p);
+    return make_uint2(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16);
+}
+
+template <typename T>
+__device__ __forceinline__ void widen4(uint2 u, float* x)
+{
+    const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i]);
-    }
+    for (int i = 0; i < 4; ++i) x[i] = to_f32(e[i]);
 }
 
 template <typename C>
-__device__ __forceinline__ void store8(C* p, const float (&x)[8])
+__device__ __forceinline__ void store4(C* p, const float* x)
 {
-    uint4 u;
+    uint2 u;
     C* e = reinterpret_cast<C*>(&u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f32<C>(x[i]);
-    *reinterpret_cast<uint4*>(p) = u;
+    for (int i = 0; i < 4; ++i) e[i] = from_f32<C>(x[i]);
+    *reinterpret_cast<uint2*>(p) = u;
 }
 
-// grid (rows, parts), 4 warps: the row's heads are dealt to the row's warps. A head is HD / 8 lanes of 8
-// consecutive elements, so a rotation pair sits rope_half / 8 lanes apart.
-template <typename T, typename C, int HD>
+// A warp handles one row and every per_row-th group of its heads (PER heads at once). A lane holds two runs of four elements of
+// a head, the two sides of its rotation pairs (c and c + rope_half), so rotating needs no exchange; lanes past the rotated
+// part hold two runs of what passes unchanged. What belongs to the row (its sequence, page, rotation) is looked up once.
+// Bound by the bytes for a long batch, whose loads are U groups deep per warp, and by latency for single tokens,
+// whose head groups each get a warp.
+template <typename T, typename C, int HD, bool VEC>
 __global__ void __launch_bounds__(128) paged_post_kernel(const PagedPostArgs a)
 {
     constexpr int L = HD / 8;                            // lanes of one head
     constexpr int PER = 32 / L;                          // heads a warp handles at once
+    constexpr int U = 4;                                 // groups in flight
     pdl_trigger();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int row = blockIdx.x;
-    const int sub = lane % L, c0 = sub * 8;
-    const int R = a.rope_half;
+    const int lane = threadIdx.x & 31, sub = lane % L;
+    const int item = blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int row = item / a.per_row, part = item - row * a.per_row;
     const exl3_paged_desc& b = a.b;
+    if (row >= b.rows) return;
+    const int R = a.rope_half;
+    const bool rotated = sub < R / 4;
+    const int c0 = rotated ? 4 * sub : R + 4 * sub;      // past the rotated part: 2 R + 4 (sub - R / 4)
+    const int c1 = rotated ? c0 + R : c0 + HD / 2 - R;
     pdl_wait();
     const int s = seq_of_row(b.cu_rows, b.seqs, row, lane);
     const int pos = b.lens[s] - b.cu_rows[s + 1] + row;
-    const bool pad = pos < 0;
-    const bool known = pos < a.rope_rows;
+    const bool pad = pos < 0, known = pos < a.rope_rows;
     const int page = page_of(b, s, pos);
-    if (!pad && (!known || page < 0) && threadIdx.x == 0) atomicOr(a.status, kStatusPagedRange);
-    const bool rotated = c0 < 2 * R;
-    float co[8] = {}, si[8] = {};
-    if (rotated && !pad && known) {
-        const size_t at = (size_t)pos * R + (c0 < R ? c0 : c0 - R);
-        *reinterpret_cast<float4*>(co) = *reinterpret_cast<const float4*>(a.cos_t + at);
-        *reinterpret_cast<float4*>(co + 4) = *reinterpret_cast<const float4*>(a.cos_t + at + 4);
-        *reinterpret_cast<float4*>(si) = *reinterpret_cast<const float4*>(a.sin_t + at);
-        *reinterpret_cast<float4*>(si + 4) = *reinterpret_cast<const float4*>(a.sin_t + at + 4);
+    if (!pad && (!known || page < 0) && lane == 0 && part == 0) atomicOr(a.status, kStatusPagedRange);
+    const bool append = !pad && known && page >= 0, has_q = !pad && known;
+    float co[4] = {}, si[4] = {};
+    if (rotated && has_q) {
+        *reinterpret_cast<float4*>(co) = *reinterpret_cast<const float4*>(a.cos_t + (size_t)pos * R + c0);
+        *reinterpret_cast<float4*>(si) = *reinterpret_cast<const float4*>(a.sin_t + (size_t)pos * R + c0);
     }
-    const int partner = c0 < R ? lane + R / 8 : lane - R / 8;
-    const int heads = a.hq + 2 * b.hkv;
-    const int stride = gridDim.y * 4 * PER;
-    for (int h0 = (blockIdx.y * 4 + warp) * PER; h0 < heads; h0 += stride) {
-        const int h = h0 + lane / L;
-        const bool live = h < heads;
-        const bool is_q = h < a.hq, is_k = !is_q && h < a.hq + b.hkv;
-        float x[8] = {};
-        if (live) {
-            const T* src = is_q ? static_cast<const T*>(a.q) + row * a.sq + (size_t)h * HD
-                         : is_k ? static_cast<const T*>(a.k) + row * a.sk + (size_t)(h - a.hq) * HD
-                                : static_cast<const T*>(a.v) + row * a.sv + (size_t)(h - a.hq - b.hkv) * HD;
-            load8(src + c0, a.vec, x);
+    uint2 wq0{}, wq1{}, wk0{}, wk1{};
+    if (a.qw) {
+        wq0 = load4<T, false>(static_cast<const T*>(a.qw) + c0);
+        wq1 = load4<T, false>(static_cast<const T*>(a.qw) + c1);
+    }
+    if (a.kw) {
+        wk0 = load4<T, false>(static_cast<const T*>(a.kw) + c0);
+        wk1 = load4<T, false>(static_cast<const T*>(a.kw) + c1);
+    }
+    const int heads = a.hq + 2 * b.hkv, stride = a.per_row * PER;
+    const T* const q = static_cast<const T*>(a.q) + row * a.sq;
+    const T* const k = static_cast<const T*>(a.k) + row * a.sk - (size_t)a.hq * HD;
+    const T* const v = static_cast<const T*>(a.v) + row * a.sv - (size_t)(a.hq + b.hkv) * HD;
+    C* const qo = static_cast<C*>(a.q_out) + (size_t)row * a.hq * HD;
+    const size_t slot = ((size_t)max(page, 0) * b.hkv * b.page_size + (pos & (b.page_size - 1))) * HD;
+    for (int g0 = part * PER; g0 < heads; g0 += U * stride) {
+        uint2 in[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = min(g0 + u * stride + lane / L, heads - 1);
+            const T* src = (h < a.hq ? q : h < a.hq + b.hkv ? k : v) + (size_t)h * HD;
+            in[u][0] = load4<T, VEC>(src + c0);
+            in[u][1] = load4<T, VEC>(src + c1);
         }
-        const T* w = static_cast<const T*>(is_q ? a.qw : a.kw);
-        float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+        for (int u = 0; u < U; ++u) {
+            const int h = g0 + u * stride + lane / L;
+            const bool live = h < heads, is_q = h < a.hq, is_k = !is_q && h < a.hq + b.hkv;
+            float x[8], y[8];
+            widen4<T>(in[u][0], x);
+            widen4<T>(in[u][1], x + 4);
+            float ss = 0.f;
 #pragma unroll
-        for (int o = 1; o < L; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (live && (is_q || is_k) && w) {
-            const float inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
+            for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * to_f32(w[c0 + i]);
-        }
-        float y[8];
+            for (int o = 1; o < L; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (is_q ? a.qw != nullptr : is_k && a.kw) {
+                const float inv = rsqrtf(ss / (float)HD + a.eps);
+                float w[8];
+                widen4<T>(make_uint2(is_q ? wq0.x : wk0.x, is_q ? wq0.y : wk0.y), w);
+                widen4<T>(make_uint2(is_q ? wq1.x : wk1.x, is_q ? wq1.y : wk1.y), w + 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float o = __shfl_sync(0xffffffffu, x[i], rotated ? partner : lane);
-            y[i] = !rotated ? x[i] : c0 < R ? x[i] * co[i] - o * si[i] : x[i] * co[i] + o * si[i];
-        }
-        if (!live) continue;
-        if (is_q) {
-            if (pad || !known)
+                for (int i = 0; i < 8; ++i) x[i] *= inv * w[i];
+            }
+            if (rotated && (is_q || is_k)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    y[i] = x[i] * co[i] - x[i + 4] * si[i];
+                    y[i + 4] = x[i + 4] * co[i] + x[i] * si[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = x[i];
+            }
+            if (is_q && !has_q)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = 0.f;
-            store8(static_cast<C*>(a.q_out) + ((size_t)row * a.hq + h) * HD + c0, y);
-        } else if (!pad && known && page >= 0) {
-            const int hk = h - a.hq - (is_k ? 0 : b.hkv);
-            const size_t at = (((size_t)page * b.hkv + hk) * b.page_size + (pos & (b.page_size - 1))) * HD + c0;
-            if (is_k) store8(static_cast<C*>(b.k_pages) + at, y);
-            else store8(static_cast<C*>(b.v_pages) + at, x);
+            C* dst = is_q ? qo + (size_t)h * HD
+                          : static_cast<C*>(is_k ? b.k_pages : b.v_pages) + slot + (size_t)(h - a.hq - (is_k ? 0 : b.hkv)) * b.page_size * HD;
+            if (live && (is_q || append)) {
+                store4(dst + c0, y);
+                store4(dst + c1, y + 4);
+            }
         }
     }
 }
 
-template <typename T, typename C>
+template <typename T, typename C, bool VEC>
 static int launch_post(const PagedPostArgs& a, dim3 grid, cudaStream_t s)
 {
-    return a.b.head_dim == 128 ? launch_pdl(paged_post_kernel<T, C, 128>, grid, dim3(128), 0, s, a)
-                               : launch_pdl(paged_post_kernel<T, C, 64>, grid, dim3(128), 0, s, a);
+    return a.b.head_dim == 128 ? launch_pdl(paged_post_kernel<T, C, 128, VEC>, grid, dim3(128), 0, s, a)
+                               : launch_pdl(paged_post_kernel<T, C, 64, VEC>, grid, dim3(128), 0, s, a);
+}
+
+template <typename T>
+static int launch_post(const PagedPostArgs& a, bool vec, dim3 grid, cudaStream_t s)
+{
+    if (a.b.dtype == EXL3_F16) return vec ? launch_post<T, __half, true>(a, grid, s) : launch_post<T, __half, false>(a, grid, s);
+    return vec ? launch_post<T, __nv_bfloat16, true>(a, grid, s) : launch_post<T, __nv_bfloat16, false>(a, grid, s);
 }
 
 }  // namespace exl3
@@ -172,15 +210,16 @@ extern "C" int exl3_paged_qkv_post(const exl3_paged_desc* batch, const void* q, 
     a.cos_t = cos_table; a.sin_t = sin_table;
     a.q_out = q_out; a.status = status; a.eps = eps;
     a.hq = hq; a.rope_rows = rope_rows; a.rope_half = rope_half;
-    a.vec = aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && q_stride % 8 == 0 && k_stride % 8 == 0 &&
-            v_stride % 8 == 0;
-    const int per_cta = 4 * (32 / (batch->head_dim / 8));
-    const int parts = (hq + 2 * batch->hkv + per_cta - 1) / per_cta;
-    const dim3 grid(batch->rows, parts);
+    const bool vec = aligned(q, 8) && aligned(k, 8) && aligned(v, 8) && q_stride % 4 == 0 && k_stride % 4 == 0 && v_stride % 4 == 0;
+    // A row's warps: one for every four groups (one round of loads) while that fits the SMs' warp slots, then fewer and longer
+    // ones. Measured at 56 heads of 128, us with 1 / 2 / 7 / 28 warps a row: 1 row 10.5 / 6.8 / 3.2 / 3.1, 600 rows 12.4 /
+    // 11.2 / 6.8 / 15.2, 3428 rows 24.1 / 25.7 / 28.2 / 83.9.
+    const int per = 32 / (batch->head_dim / 8), groups = (hq + 2 * batch->hkv + per - 1) / per;
+    const int warps = 32 * device_sm_count();
+    a.per_row = std::max(1, std::min((groups + 3) / 4, warps / batch->rows));
+    const long long items = (long long)batch->rows * a.per_row;
+    if ((items + 3) / 4 > 0x7fffffffll || items > 0x7fffffffll) return EXL3_E_SHAPE;
+    const dim3 grid((unsigned)((items + 3) / 4));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (in_dtype == EXL3_F16)
-        return batch->dtype == EXL3_F16 ? launch_post<__half, __half>(a, grid, s)
-                                        : launch_post<__half, __nv_bfloat16>(a, grid, s);
-    return batch->dtype == EXL3_F16 ? launch_post<__nv_bfloat16, __half>(a, grid, s)
-                                    : launch_post<__nv_bfloat16, __nv_bfloat16>(a, grid, s);
+    return in_dtype == EXL3_F16 ? launch_post<__half>(a, vec, grid, s) : launch_post<__nv_bfloat16>(a, vec, grid, s);
 }

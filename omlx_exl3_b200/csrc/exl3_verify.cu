@@ -23,8 +23,9 @@
 namespace exl3 {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kVerifyThreads = 512;
-constexpr int kVerifyWarps = kVerifyThreads / 32;
+constexpr int kStatThreads = 128, kStatWarps = kStatThreads / 32;
+constexpr int kStatPer = 32;                          // columns a thread keeps in registers
+constexpr int kDecideWarps = 16;                      // most of a CTA
 constexpr int kVerifyCluster = 8;
 
 struct VerifyArgs {
@@ -40,18 +41,6 @@ struct VerifyArgs {
     int rows, seqs, n, max_drafts, chunks;
 };
 
-// The sequence of draft i: sequence s holds drafts cu_rows[s] - s .. cu_rows[s + 1] - s - 2.
-__device__ __forceinline__ int seq_of_draft(const int32_t* cu_rows, int seqs, int i)
-{
-    int lo = 0, hi = seqs - 1;                        // the first s with i < cu_rows[s + 1] - s - 1
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (i < cu_rows[mid + 1] - mid - 1) hi = mid;
-        else lo = mid + 1;
-    }
-    return lo;
-}
-
 // (value, column) of the larger value, of the first column among equals.
 __device__ __forceinline__ void take_first(float& v, int& i, float ov, int oi)
 {
@@ -62,43 +51,48 @@ __device__ __forceinline__ void take_first(float& v, int& i, float ov, int oi)
 }
 
 // ------------------------------------------------------------------------------ statistics
-// PER columns per thread. The row's columns from its first 16-byte boundary on go to the chunks as whole vectors; the few
+// Small CTAs, so that some load while others reduce. The row's columns from its first 16-byte boundary on go to the chunks as whole vectors; the few
 // before it are chunk 0's, the last vector may be partial.
-template <typename T, int PER>
-__global__ void __launch_bounds__(kVerifyThreads) verify_stats_kernel(const VerifyArgs a)
+template <typename T>
+__global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const VerifyArgs a)
 {
-    constexpr int VEC = 16 / sizeof(T), N = PER / VEC;
-    __shared__ float sv[kVerifyWarps];
-    __shared__ int si[kVerifyWarps];
+    constexpr int PER = kStatPer, VEC = 16 / sizeof(T), N = PER / VEC;
+    __shared__ float sv[kStatWarps];
+    __shared__ int si[kStatWarps];
     pdl_trigger();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = blockIdx.x / a.chunks, chunk = blockIdx.x - r * a.chunks;
     const bool is_draft = r >= a.rows;
-    float temp = 1.f;
-    if (a.temperature) {
-        const int s = is_draft ? seq_of_draft(a.cu_rows, a.seqs, r - a.rows) : seq_of_row(a.cu_rows, a.seqs, r, lane);
-        temp = a.temperature[s];
-    }
-    const bool greedy = !(temp > 0.f);
-    if (greedy && is_draft) return;                   // q is one-hot: the row is not looked at
     const T* x = is_draft ? static_cast<const T*>(a.draft) + (r - a.rows) * a.draft_ld
                           : static_cast<const T*>(a.target) + r * a.target_ld;
     const int head = min(a.n, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-    const int first = head + chunk * (kVerifyThreads * PER) + tid * VEC;
+    const int first = head + chunk * (kStatThreads * PER) + tid * VEC;
+    uint4 w[N];
+    auto fetch = [&]() {                              // whole vectors; the row's last may be partial
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int at = first + k * kStatThreads * VEC;
+            if (at + VEC <= a.n) w[k] = *reinterpret_cast<const uint4*>(x + at);
+        }
+    };
+    // a target row's logits are on their way while its temperature is looked up
+    if (!is_draft) fetch();
+    float temp = 1.f;
+    if (a.temperature)
+        temp = a.temperature[is_draft ? seq_of_row<1>(a.cu_rows, a.seqs, r - a.rows, lane) : seq_of_row(a.cu_rows, a.seqs, r, lane)];
+    const bool greedy = !(temp > 0.f);
+    if (is_draft) {
+        if (greedy) return;                           // q is one-hot: the row is not looked at
+        fetch();
+    }
     float v[PER + 1];
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const int at = first + k * kVerifyThreads * VEC;
-        if (at + VEC <= a.n) {
-            const uint4 w = *reinterpret_cast<const uint4*>(x + at);
-            const T* e = reinterpret_cast<const T*>(&w);
+        const int at = first + k * kStatThreads * VEC;
+        const T* e = reinterpret_cast<const T*>(&w[k]);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[k * VEC + i] = to_f32(e[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[k * VEC + i] = at + i < a.n ? to_f32(x[at + i]) : -INFINITY;
-        }
+        for (int i = 0; i < VEC; ++i) v[k * VEC + i] = at + VEC <= a.n ? to_f32(e[i]) : at + i < a.n ? to_f32(x[at + i]) : -INFINITY;
     }
     v[PER] = chunk == 0 && tid < head ? to_f32(x[tid]) : -INFINITY;
     float m = v[PER];
@@ -108,9 +102,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_stats_kernel(const Veri
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) sv[warp] = m;
     __syncthreads();
-    m = sv[lane & (kVerifyWarps - 1)];
+    m = sv[lane & (kStatWarps - 1)];
 #pragma unroll
-    for (int o = kVerifyWarps / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = kStatWarps / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float base = m == -INFINITY ? 0.f : m, c = (greedy ? 1.f : 1.f / temp) * kLog2e;
     float s0 = ex2((v[PER] - base) * c), s1 = 0.f;
 #pragma unroll
@@ -123,7 +117,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_stats_kernel(const Veri
     if (greedy) {
 #pragma unroll
         for (int i = PER - 1; i >= 0; --i)
-            if (v[i] == m) at = first + (i / VEC) * kVerifyThreads * VEC + i % VEC;
+            if (v[i] == m) at = first + (i / VEC) * kStatThreads * VEC + i % VEC;
         if (chunk == 0 && tid < head && v[PER] == m) at = tid;
 #pragma unroll
         for (int o = 16; o; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
@@ -137,7 +131,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_stats_kernel(const Veri
     if (tid == 0) {
         float sum = 0.f;
         int col = 0x7fffffff;
-        for (int w = 0; w < kVerifyWarps; ++w) {
+        for (int w = 0; w < kStatWarps; ++w) {
             sum += sv[w];
             col = min(col, si[w]);
         }
@@ -159,35 +153,47 @@ __device__ __forceinline__ float joined(float s0, float m0, float s1, float m1, 
     return (m0 == -INFINITY ? s0 : s0 * ex2((m0 - now) * c)) + (m1 == -INFINITY ? s1 : s1 * ex2((m1 - now) * c));
 }
 
-__device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, int row, float c, int lane)
-{
+struct PartStat {                                     // of some of a row's chunks
     float m = -INFINITY, s = 0.f;
-    int at = 0x7fffffff;
-    for (int k = lane; k < a.chunks; k += 32) {
-        const float4 w = __ldcg(a.stats + (size_t)row * a.chunks + k);
-        const float now = fmaxf(m, w.x);
-        s = joined(s, m, w.y, w.x, now, c);
-        take_first(m, at, w.x, __float_as_int(w.z));
+    int first = 0x7fffffff;
+    __device__ __forceinline__ void join(float om, float os, int of, float c)
+    {
+        s = joined(s, m, os, om, fmaxf(m, om), c);
+        take_first(m, first, om, of);
+    }
+};
+
+// Statistics of one or (b >= 0) two rows from their chunks', by a warp; both rows' chunks are loaded together.
+__device__ __forceinline__ void row_stats(const VerifyArgs& a, long long ra, long long rb, float c, int lane, RowStat& outa, RowStat& outb)
+{
+    PartStat p[2];
+    for (int k0 = 0; k0 < a.chunks; k0 += 64) {
+        float4 w[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int k = k0 + 32 * j + lane;
+                const long long row = i ? rb : ra;
+                w[i][j] = row >= 0 && k < a.chunks ? __ldcg(a.stats + row * a.chunks + k)
+                                                   : make_float4(-INFINITY, 0.f, __int_as_float(0x7fffffff), 0.f);
+            }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) p[i].join(w[i][j].x, w[i][j].y, __float_as_int(w[i][j].z), c);
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o);
-        const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-        const float now = fmaxf(m, om);
-        s = joined(s, m, os, om, now, c);
-        take_first(m, at, om, oa);
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+            p[i].join(__shfl_xor_sync(0xffffffffu, p[i].m, o), __shfl_xor_sync(0xffffffffu, p[i].s, o),
+                      __shfl_xor_sync(0xffffffffu, p[i].first, o), c);
+        RowStat& r = i ? outb : outa;
+        r.m = p[i].m == -INFINITY ? 0.f : p[i].m;
+        r.inv = p[i].s > 0.f ? 1.f / p[i].s : 0.f;
+        r.first = p[i].first;
     }
-    RowStat r;
-    r.m = m == -INFINITY ? 0.f : m;
-    r.inv = s > 0.f ? 1.f / s : 0.f;
-    r.first = at;
-    return r;
-}
-
-template <typename T>
-__device__ __forceinline__ float prob_of(const T* x, long long v, const RowStat& r, float c)
-{
-    return ex2((to_f32(x[v]) - r.m) * c) * r.inv;
 }
 
 struct Verdict {                                      // of one row, by the warp that looked at it
@@ -198,16 +204,16 @@ struct Verdict {                                      // of one row, by the warp
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kVerifyThreads) verify_decide_kernel(const VerifyArgs a)
+__global__ void __launch_bounds__(32 * kDecideWarps) verify_decide_kernel(const VerifyArgs a)
 {
     constexpr int VEC = 16 / sizeof(T);
-    __shared__ Verdict row_s[kVerifyWarps];
-    __shared__ float bv[kVerifyWarps];
-    __shared__ int bi[kVerifyWarps];
+    __shared__ Verdict row_s[kDecideWarps];
+    __shared__ float bv[kDecideWarps];
+    __shared__ int bi[kDecideWarps];
     __shared__ float2 mine[2];                        // this CTA's winner of a pass (value, column)
     pdl_trigger();
     pdl_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthr = blockDim.x, nwarp = nthr >> 5;
     const int rank = (int)cluster_rank();
     const int s = blockIdx.x / kVerifyCluster;
     const int lo = a.cu_rows[s], hi = a.cu_rows[s + 1];
@@ -218,39 +224,49 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_decide_kernel(const Ver
     const int judged = sane ? hi - lo - 1 : 0;        // drafts of this sequence
     const int limit = min(judged, a.max_drafts);
 
+    // the noise is not known to any cache yet, and its columns do not depend on the verdict
+    if (sane && !greedy)
+        for (int v = (rank * nthr + tid) * 32; v < a.n; v += nthr * kVerifyCluster * 32)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(a.noise + s * a.noise_ld + v));
+
     // rows in order, a warp each, until one does not stand (the first CTA goes on: accept_prob is every draft's)
     int n_acc = -1;
     Verdict at{};
-    for (int j0 = 0; sane && j0 <= judged; j0 += kVerifyWarps) {
+    for (int j0 = 0; sane && j0 <= judged; j0 += nwarp) {
         const int j = j0 + warp;
         if (j <= judged) {
             const T* tr = static_cast<const T*>(a.target) + (lo + j) * a.target_ld;
             Verdict v{};
-            v.p = row_stat(a, lo + j, c, lane);
-            if (j < judged) {
-                const int i = lo + j - s;
+            const bool has = j < judged, two = has && a.draft && !greedy;
+            const int i = lo + j - s;
+            float u = 0.f, xt = 0.f, xd = 0.f;
+            if (has) {
                 v.token = a.tokens[i];
-                const bool in = v.token >= 0 && v.token < a.n;
+                u = a.u[i];
+            }
+            const bool in = has && v.token >= 0 && v.token < a.n;
+            if (in) {
+                xt = to_f32(tr[v.token]);
+                if (two) xd = to_f32((static_cast<const T*>(a.draft) + i * a.draft_ld)[v.token]);
+            }
+            row_stats(a, lo + j, two ? (long long)a.rows + i : -1, c, lane, v.p, v.q);
+            if (has) {
                 float p = 0.f, q = 1.f;
                 if (greedy) {
                     p = in && v.token == v.p.first && v.p.inv > 0.f ? 1.f : 0.f;
                 } else {
-                    if (in) p = prob_of(tr, v.token, v.p, c);
-                    if (a.draft) {
-                        const T* dr = static_cast<const T*>(a.draft) + i * a.draft_ld;
-                        v.q = row_stat(a, a.rows + i, c, lane);
-                        q = in ? prob_of(dr, v.token, v.q, c) : 0.f;
-                    }
+                    if (in) p = ex2((xt - v.p.m) * c) * v.p.inv;
+                    if (two) q = in ? ex2((xd - v.q.m) * c) * v.q.inv : 0.f;
                 }
                 v.prob = q > 0.f ? fminf(p / q, 1.f) : (p > 0.f ? 1.f : 0.f);
-                v.stands = j < limit && a.u[i] < v.prob;
+                v.stands = j < limit && u < v.prob;
                 if (rank == 0 && lane == 0) a.prob[i] = v.prob;
             }
             if (lane == 0) row_s[warp] = v;
         }
         __syncthreads();
         if (n_acc < 0)
-            for (int k = 0; k < kVerifyWarps && j0 + k <= judged; ++k)
+            for (int k = 0; k < nwarp && j0 + k <= judged; ++k)
                 if (!row_s[k].stands) {
                     n_acc = j0 + k;
                     at = row_s[k];
@@ -276,14 +292,14 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_decide_kernel(const Ver
             auto consider = [&](int v, float x, float d, float noise) {
                 float w = ex2((x - at.p.m) * c) * at.p.inv;
                 if (pass == 0) w -= dr ? ex2((d - at.q.m) * c) * at.q.inv : (v == at.token ? 1.f : 0.f);
-                const float score = w / noise;
-                if (score > best) {                   // columns come in rising order per thread
-                    best = score;
+                if (w > best * noise) {               // w / noise > best; columns come in rising order per thread
+                    best = w / noise;
                     idx = v;
                 }
             };
-            const int threads = kVerifyThreads * kVerifyCluster, me = rank * kVerifyThreads + tid;
+            const int threads = nthr * kVerifyCluster, me = rank * nthr + tid;
             const int whole = vec ? a.n / VEC * VEC : 0;
+#pragma unroll 2
             for (int v = me * VEC; v < whole; v += threads * VEC) {
                 const uint4 xr = *reinterpret_cast<const uint4*>(tr + v);
                 const uint4 dx = dr && pass == 0 ? *reinterpret_cast<const uint4*>(dr + v) : make_uint4(0, 0, 0, 0);
@@ -307,7 +323,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_decide_kernel(const Ver
             }
             __syncthreads();
             if (tid == 0) {
-                for (int w = 1; w < kVerifyWarps; ++w) take_first(best, idx, bv[w], bi[w]);
+                for (int w = 1; w < nwarp; ++w) take_first(best, idx, bv[w], bi[w]);
                 mine[pass] = make_float2(best, __int_as_float(idx));
             }
             cluster_sync_all();
@@ -330,36 +346,25 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_decide_kernel(const Ver
     }
     if (rank == 0) {
         long long* out = a.out + (size_t)s * (a.max_drafts + 1);
-        for (int j = tid; j <= a.max_drafts; j += kVerifyThreads)
+        for (int j = tid; j <= a.max_drafts; j += nthr)
             out[j] = j < n_acc ? a.tokens[lo + j - s] : j == n_acc ? next : -1;
         if (tid == 0) a.count[s] = n_acc + 1;
     }
 }
 
-// 32 columns a thread, or 8 where that leaves SMs without a CTA (a sequence or two).
-struct VerifyPlan {
-    int per, chunks;
-    long long stat_rows;
-};
+static int verify_chunks(int n) { return (n + kStatPer * kStatThreads - 1) / (kStatPer * kStatThreads); }
 
-static VerifyPlan verify_plan(int rows, int seqs, int n)
-{
-    VerifyPlan p;
-    p.stat_rows = 2ll * rows - seqs;
-    p.per = p.stat_rows * (n / (32 * kVerifyThreads) + 1) < 2 * device_sm_count() ? 8 : 32;
-    p.chunks = (n + p.per * kVerifyThreads - 1) / (p.per * kVerifyThreads);
-    return p;
-}
+static size_t verify_bytes(int rows, int seqs, int n) { return (size_t)(2ll * rows - seqs) * verify_chunks(n) * sizeof(float4); }
 
 template <typename T>
-static int launch_verify(const VerifyArgs& a, int per, cudaStream_t s)
+static int launch_verify(const VerifyArgs& a, cudaStream_t s)
 {
     const long long ctas = (long long)(a.rows + (a.draft ? a.rows - a.seqs : 0)) * a.chunks;
     if (ctas > 0x7fffffffll) return EXL3_E_SHAPE;
-    const int e = per == 8 ? launch_pdl(verify_stats_kernel<T, 8>, dim3((unsigned)ctas), dim3(kVerifyThreads), 0, s, a)
-                           : launch_pdl(verify_stats_kernel<T, 32>, dim3((unsigned)ctas), dim3(kVerifyThreads), 0, s, a);
-    if (e) return e;
-    return launch_pdl_cluster(verify_decide_kernel<T>, dim3(a.seqs * kVerifyCluster), dim3(kVerifyThreads), 0, kVerifyCluster, s, a);
+    if (int e = launch_pdl(verify_stats_kernel<T>, dim3((unsigned)ctas), dim3(kStatThreads), 0, s, a)) return e;
+    // wide CTAs while every cluster has SMs of its own, then narrower ones so that all are resident at once
+    const int threads = a.seqs * kVerifyCluster <= device_sm_count() ? 512 : 256;
+    return launch_pdl_cluster(verify_decide_kernel<T>, dim3(a.seqs * kVerifyCluster), dim3(threads), 0, kVerifyCluster, s, a);
 }
 
 }  // namespace exl3
@@ -375,8 +380,7 @@ extern "C" int exl3_verify_workspace(int rows, int seqs, int n, size_t* bytes)
 {
     if (!bytes) return EXL3_E_NULL;
     if (int e = check_verify(rows, seqs, n)) return e;
-    const VerifyPlan p = verify_plan(rows, seqs, n);
-    *bytes = (size_t)p.stat_rows * p.chunks * sizeof(float4);
+    *bytes = verify_bytes(rows, seqs, n);
     return EXL3_OK;
 }
 
@@ -397,8 +401,7 @@ extern "C" int exl3_verify_drafts(const void* target, long long target_ld, const
         !aligned(temperature, 4) || !aligned(workspace, 16))
         return EXL3_E_ALIGN;
     if (int e = check_device()) return e;
-    const VerifyPlan p = verify_plan(rows, seqs, n);
-    if (workspace_bytes < (size_t)p.stat_rows * p.chunks * sizeof(float4)) return EXL3_E_WORKSPACE;
+    if (workspace_bytes < verify_bytes(rows, seqs, n)) return EXL3_E_WORKSPACE;
     VerifyArgs a{};
     a.target = target; a.draft = draft;
     a.target_ld = target_ld; a.draft_ld = draft_ld; a.noise_ld = noise_ld;
@@ -406,11 +409,11 @@ extern "C" int exl3_verify_drafts(const void* target, long long target_ld, const
     a.out = tokens_out; a.count = count; a.prob = accept_prob;
     a.stats = static_cast<float4*>(workspace);
     a.rows = rows; a.seqs = seqs; a.n = n; a.max_drafts = max_drafts;
-    a.chunks = p.chunks;
+    a.chunks = verify_chunks(n);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-    case EXL3_F16: return launch_verify<__half>(a, p.per, s);
-    case EXL3_BF16: return launch_verify<__nv_bfloat16>(a, p.per, s);
-    default: return launch_verify<float>(a, p.per, s);
+    case EXL3_F16: return launch_verify<__half>(a, s);
+    case EXL3_BF16: return launch_verify<__nv_bfloat16>(a, s);
+    default: return launch_verify<float>(a, s);
     }
 }
