@@ -14,6 +14,7 @@
 #include "exl3_b200.h"
 #include "exl3_common.cuh"
 #include "exl3_paged.cuh"
+#include "exl3_paged_math.cuh"
 
 namespace exl3 {
 
@@ -175,13 +176,6 @@ struct PaSched {
         return true;
     }
 };
-
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // exp2((m - top) * c), 0 for a row that has seen nothing (m = -inf).
 __device__ __forceinline__ float pa_weight(float m, float top, float c)

@@ -13,11 +13,13 @@
 // another order of summation; the race depends on each w alone.
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "exl3_b200.h"
 #include "exl3_common.cuh"
 #include "exl3_host.h"
 #include "exl3_paged.cuh"
-#include "exl3_paged_sched.cuh"
+#include "exl3_paged_math.cuh"
 #include "exl3_tc.cuh"
 
 namespace exl3 {
@@ -73,7 +75,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int at = first + k * kStatThreads * VEC;
-            if (at + VEC <= a.n) w[k] = *reinterpret_cast<const uint4*>(x + at);
+            w[k] = at + VEC <= a.n ? *reinterpret_cast<const uint4*>(x + at) : make_uint4(0, 0, 0, 0);
         }
     };
     // a target row's logits are on their way while its temperature is looked up
@@ -89,15 +91,23 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
     float v[PER + 1];
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const int at = first + k * kStatThreads * VEC;
         const T* e = reinterpret_cast<const T*>(&w[k]);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[k * VEC + i] = at + VEC <= a.n ? to_f32(e[i]) : at + i < a.n ? to_f32(x[at + i]) : -INFINITY;
+        for (int i = 0; i < VEC; ++i) v[k * VEC + i] = to_f32(e[i]);
+    }
+    if (head + (chunk + 1) * (kStatThreads * PER) > a.n) {             // the row ends in this chunk
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int at = first + k * kStatThreads * VEC;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (at + VEC > a.n) v[k * VEC + i] = at + i < a.n ? to_f32(x[at + i]) : -INFINITY;
+        }
     }
     v[PER] = chunk == 0 && tid < head ? to_f32(x[tid]) : -INFINITY;
     float m = v[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) m = fmaxf(m, v[i]);
+    for (int i = 0; i < PER; i += 2) m = max3(m, v[i], v[i + 1]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) sv[warp] = m;
@@ -106,12 +116,17 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
 #pragma unroll
     for (int o = kStatWarps / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float base = m == -INFINITY ? 0.f : m, c = (greedy ? 1.f : 1.f / temp) * kLog2e;
-    float s0 = ex2((v[PER] - base) * c), s1 = 0.f;
+    // the maximum is taken off before scaling: the lowest value of the type scaled by 1 / T would overflow
+    const uint64_t c2 = f2(c, c), zero = f2(0.f, 0.f), off = f2(-base, -base);
+    uint64_t s2 = f2(ex2((v[PER] - base) * c), 0.f);
 #pragma unroll
     for (int i = 0; i < PER; i += 2) {
-        s0 += ex2((v[i] - base) * c);
-        s1 += ex2((v[i + 1] - base) * c);
+        float e0, e1;
+        f2_get(f2_fma(f2_add(f2(v[i], v[i + 1]), off), c2, zero), e0, e1);
+        s2 = f2_add(s2, f2(ex2(e0), ex2(e1)));
     }
+    float s0, s1;
+    f2_get(s2, s0, s1);
     const float s = warp_sum(s0 + s1);
     int at = 0x7fffffff;
     if (greedy) {
@@ -285,36 +300,60 @@ __global__ void __launch_bounds__(32 * kDecideWarps) verify_decide_kernel(const 
         const T* dr = a.draft && rejected ? static_cast<const T*>(a.draft) + (lo + n_acc - s) * a.draft_ld : nullptr;
         const float* e = a.noise + s * a.noise_ld;
         const bool vec = ((reinterpret_cast<uintptr_t>(tr) | reinterpret_cast<uintptr_t>(dr) | reinterpret_cast<uintptr_t>(e)) & 15) == 0;
+        const int threads = nthr * kVerifyCluster, me = rank * nthr + tid;
+        const int banned = at.token >= 0 && at.token < a.n ? (int)at.token : -1;
+        // Columns of this thread in rising order; MODE 0: w = p, 1: w = p - q, 2: w = p but for the rejected token (one-hot q).
+        // w / noise > best is asked as w > best * noise; the division is for the few that pass.
+        auto race = [&](auto mode, float& best, int& idx) {
+            constexpr int MODE = decltype(mode)::value;
+            auto weight = [&](int v, float x, float d) {
+                // products rounded before the difference: where q is p, w is zero
+                float w = __fmul_rn(ex2((x - at.p.m) * c), at.p.inv);
+                if (MODE == 1) w = __fsub_rn(w, __fmul_rn(ex2((d - at.q.m) * c), at.q.inv));
+                if (MODE == 2 && v == banned) w = 0.f;
+                return w;
+            };
+            const int whole = vec ? a.n / VEC * VEC : 0;
+#pragma unroll 1
+            for (int v = me * VEC; v < whole; v += threads * VEC) {
+                const uint4 xr = *reinterpret_cast<const uint4*>(tr + v);
+                const uint4 dx = MODE == 1 ? *reinterpret_cast<const uint4*>(dr + v) : make_uint4(0, 0, 0, 0);
+                float nz[VEC], w[VEC];
+#pragma unroll
+                for (int i = 0; i < VEC; i += 4) *reinterpret_cast<float4*>(nz + i) = *reinterpret_cast<const float4*>(e + v + i);
+                const T* xe = reinterpret_cast<const T*>(&xr);
+                const T* de = reinterpret_cast<const T*>(&dx);
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    w[i] = weight(v + i, to_f32(xe[i]), to_f32(de[i]));
+                    any |= w[i] > best * nz[i];
+                }
+                if (any) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i)
+                        if (w[i] > best * nz[i]) {
+                            best = w[i] / nz[i];
+                            idx = v + i;
+                        }
+                }
+            }
+#pragma unroll 4
+            for (int v = whole + me; v < a.n; v += threads) {
+                const float w = weight(v, to_f32(tr[v]), MODE == 1 ? to_f32(dr[v]) : 0.f), nz = e[v];
+                if (w > best * nz) {
+                    best = w / nz;
+                    idx = v;
+                }
+            }
+        };
         // first the residual, then (where that is zero everywhere) p itself
         for (int pass = rejected ? 0 : 1; pass < 2; ++pass) {
             float best = 0.f;
             int idx = 0x7fffffff;
-            auto consider = [&](int v, float x, float d, float noise) {
-                float w = ex2((x - at.p.m) * c) * at.p.inv;
-                if (pass == 0) w -= dr ? ex2((d - at.q.m) * c) * at.q.inv : (v == at.token ? 1.f : 0.f);
-                if (w > best * noise) {               // w / noise > best; columns come in rising order per thread
-                    best = w / noise;
-                    idx = v;
-                }
-            };
-            const int threads = nthr * kVerifyCluster, me = rank * nthr + tid;
-            const int whole = vec ? a.n / VEC * VEC : 0;
-#pragma unroll 2
-            for (int v = me * VEC; v < whole; v += threads * VEC) {
-                const uint4 xr = *reinterpret_cast<const uint4*>(tr + v);
-                const uint4 dx = dr && pass == 0 ? *reinterpret_cast<const uint4*>(dr + v) : make_uint4(0, 0, 0, 0);
-                float4 nz[VEC / 4];
-#pragma unroll
-                for (int i = 0; i < VEC / 4; ++i) nz[i] = *reinterpret_cast<const float4*>(e + v + 4 * i);
-                const T* xe = reinterpret_cast<const T*>(&xr);
-                const T* de = reinterpret_cast<const T*>(&dx);
-                const float* ne = reinterpret_cast<const float*>(nz);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) consider(v + i, to_f32(xe[i]), to_f32(de[i]), ne[i]);
-            }
-#pragma unroll 4
-            for (int v = whole + me; v < a.n; v += threads)
-                consider(v, to_f32(tr[v]), dr && pass == 0 ? to_f32(dr[v]) : 0.f, e[v]);
+            if (pass == 1) race(std::integral_constant<int, 0>{}, best, idx);
+            else if (dr) race(std::integral_constant<int, 1>{}, best, idx);
+            else race(std::integral_constant<int, 2>{}, best, idx);
 #pragma unroll
             for (int o = 16; o; o >>= 1) take_first(best, idx, __shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, idx, o));
             if (lane == 0) {
