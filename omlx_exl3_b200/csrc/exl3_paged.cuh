@@ -35,7 +35,7 @@ __device__ __forceinline__ int seq_of_row(const int32_t* cu_rows, int seqs, int 
 // Page of position `pos` of sequence s; -1 where the table has none or names one outside the pool.
 __device__ __forceinline__ int page_of(const exl3_paged_desc& b, int s, int pos)
 {
-    const int col = pos / b.page_size;
+    const int col = pos >> (31 - __clz(b.page_size));    // a power of two
     if (pos < 0 || col >= b.table_cols) return -1;
     const int page = b.page_table[(size_t)s * b.table_cols + col];
     return page >= 0 && page < b.num_pages ? page : -1;

@@ -216,10 +216,10 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     bool ok = true;
 
     // Tiles of the segment: tokens per tile, the second tile's only where the item has more than one tile's.
-    const int tokens = kPaRows / a.grp;
+    const int tokens = by_grp(a, kPaRows);
     struct Item { int row0, pos0, ntok[2]; bool dual; };
     auto item_of = [&](const PaSeg& g) {
-        const int tok0 = g.p0 / a.grp, ntok = min(g.rows - tok0, 2 * tokens);
+        const int tok0 = by_grp(a, g.p0), ntok = min(g.rows - tok0, 2 * tokens);
         Item i;
         i.row0 = g.start + tok0;
         i.pos0 = g.ctx + tok0;
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                 pg2 = pg3;
             }
         }
-        if (lane == 0) pa_record(a, n_seg > 0, g, n_seg > 0 ? min(2 * tokens, g.rows - g.p0 / a.grp) * a.grp : 0, tokens * a.grp);
+        if (lane == 0) pa_record(a, n_seg > 0, g, n_seg > 0 ? min(2 * tokens, g.rows - by_grp(a, g.p0)) * a.grp : 0, tokens * a.grp);
         // nothing of this CTA may still be landing when it exits
         for (uint32_t i = it > (uint32_t)P::kStages ? it - P::kStages : 0; i < it; ++i)
             if (!pa_wait(&full[i % P::kStages], (i / P::kStages) & 1, kPaExitNs)) ok = false;
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
             const bool dual = im.dual;
             const int tile = dual ? slot : 0;
             const int used = im.ntok[tile] * a.grp;
-            const int tok = r / a.grp;
+            const int tok = by_grp(a, r);
             const int pos = im.pos0 + tile * tokens + tok;
             const int limit = r < used ? min(pos + 1, g.end) : 0x7fffffff;    // positions this row sees; unused rows: any
             const bool idle = quarter * 32 >= used;                    // no row of this warp is used
@@ -711,7 +711,7 @@ int pa_launch_tiles(const PaArgs& args, cudaStream_t s)
     PaArgs a = args;
     const int tokens = kPaRows / a.grp;
     a.span = 2 * tokens * a.grp;
-    a.item = getenv("PT_ITEM") ? atoi(getenv("PT_ITEM")) : 2;
+    a.item = 2;
     auto encode = exl3_get_tensormap_encoder();
     if (!encode) return EXL3_E_CUDA;
     CUtensorMap qm, km, vm;
@@ -758,6 +758,8 @@ extern "C" int exl3_paged_attn(const exl3_paged_desc* batch, const void* q, long
     a.scale_log2 = scale * 1.4426950408889634f;
     a.hq = hq;
     a.grp = hq / batch->hkv;
+    a.grp_magic = a.grp == 1 ? 0u : (uint32_t)(((1ull << 32) + a.grp - 1) / a.grp);
+    if (!pa_list_fits(a, 8)) return EXL3_E_SHAPE;
     // Which kernel takes a sequence goes by its packed rows, which only the device knows, unless there is one sequence. A
     // batch with a row per sequence at most is taken for single tokens: one launch, right whatever the rows are.
     cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
             lj = lg.j0;
             ltab = a.b.page_table + (size_t)lg.s * a.b.table_cols;
         }
-        lpage = ltab[lpos / a.b.page_size];           // lpos < end <= table_cols * page_size
+        lpage = ltab[lpos >> (31 - __clz(a.b.page_size))];             // lpos < end <= table_cols * page_size
     };
     auto load = [&]() {
         if (lany) {
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
         int lim[NQ][2], least = 0x7fffffff;
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
-            const int p = g.p0 + 8 * t + gid, tok = p / a.grp, row = g.start + tok;
+            const int p = g.p0 + 8 * t + gid, tok = by_grp(a, p), row = g.start + tok;
             const bool live = 8 * t + gid < used && row < a.b.rows;
             const C* src = static_cast<const C*>(a.q) + row * a.q_stride + (size_t)(g.h * a.grp + (p - tok * a.grp)) * HD + 2 * tig;
 #pragma unroll
@@ -174,11 +174,11 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int q = 8 * t + 2 * tig + e;
-                lim[t][e] = q < used ? min(g.end, g.ctx + (g.p0 + q) / a.grp + 1) : 0x7fffffff;
+                lim[t][e] = q < used ? min(g.end, g.ctx + by_grp(a, g.p0 + q) + 1) : 0x7fffffff;
                 least = min(least, lim[t][e]);
             }
         }
-        if (lane == 0 && warp == 0 && (long long)g.ctx + (g.p0 + used - 1) / a.grp >= sched.cap) atomicOr(a.status, kStatusPagedRange);
+        if (lane == 0 && warp == 0 && g.ctx + by_grp(a, g.p0 + used - 1) >= sched.cap) atomicOr(a.status, kStatusPagedRange);
         float o[HD / 16][NQ][4] = {};
         float m[NQ][2], l[NQ][2];
 #pragma unroll
@@ -276,8 +276,9 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
                     for (int e = 0; e < 4; ++e)
                         merge[(warp * 8 * NQ + 8 * t + 2 * tig + (e & 1)) * S::kPad + i * 16 - c0 + gid + 8 * (e >> 1)] = o[i][t][e];
             __syncthreads();
-            for (int x = threadIdx.x; x < used * (S::kCols / 4); x += 32 * kPfWarps) {
-                const int r = x % used, quad = x / used;
+            const int r = threadIdx.x % (8 * NQ), quad = threadIdx.x / (8 * NQ);       // a thread per row and column quad
+            static_assert(8 * NQ * (S::kCols / 4) <= 32 * kPfWarps, "one pass");
+            if (r < used && quad < S::kCols / 4) {
                 float top = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < kPfWarps; ++w) top = fmaxf(top, wm[w][r]);
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
                     acc.w += y.w * f;
                 }
                 if (whole) {
-                    const int p = g.p0 + r, tok = p / a.grp, row = g.start + tok;
+                    const int p = g.p0 + r, tok = by_grp(a, p), row = g.start + tok;
                     if (row < a.b.rows) {
                         const float inv = 1.f / sum;
                         uint2 w = make_uint2(pack2<C>(acc.x * inv, acc.y * inv), pack2<C>(acc.z * inv, acc.w * inv));
@@ -328,7 +329,7 @@ static int launch_few(const PaArgs& args, cudaStream_t s)
     }
     PaArgs a = args;
     a.span = 8 * NQ;
-    a.item = getenv("PF_ITEM") ? atoi(getenv("PF_ITEM")) : 4;
+    a.item = 4;
     const int ctas = device_sm_count();
     return launch_pdl(paged_few_kernel<C, HD, NQ>, dim3(ctas), dim3(32 * kPfWarps), PfShape<HD, NQ>::kSmem, s, a);
 }

@@ -3,7 +3,7 @@
 //
 // grid (CTAs of the attention kernels, blocks of an item, lists): block x looks at the item that started in CTA x's share.
 // (One CTA, the last to finish its part, merging alone was measured first: 40 rows of 33 parts are 0.7 MB, 25 us for one
-// SM.) The time is L2 latency: the loads of E column quads and K parts are in flight at once.
+// SM.) The time is L2 latency, so a quad's parts are loaded four at a time, and by four threads where there are many.
 #include <cuda_runtime.h>
 
 #include "exl3_b200.h"
@@ -15,76 +15,110 @@
 namespace exl3 {
 
 constexpr int kPmThreads = 128;
-constexpr int kPmBlocks = 8;                          // of an item
+constexpr int kPmBlocks = 16;                         // of an item of tiles
+constexpr int kPmFewBlocks = 4;                       // of one of few rows
+
+// A column quad of an item: its tile, its row there, its place in the tile's parts.
+struct PmQuad {
+    int tile, row, at, quad;
+};
+
+template <int HD, int TILES>
+__device__ __forceinline__ PmQuad pm_quad(const PaItem& g, int e)
+{
+    const int used0 = min(g.used, g.gap);
+    PmQuad q;
+    q.tile = TILES > 1 && e >= used0 * (HD / 4) ? 1 : 0;
+    q.at = e - q.tile * used0 * (HD / 4);
+    const int used = q.tile ? g.used - used0 : used0;
+    q.quad = q.at / used;
+    q.row = q.at - q.quad * used;
+    return q;
+}
+
+// A running (m, l, O) of a column quad.
+struct PmSum {
+    float top = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    __device__ __forceinline__ void scale(float f)
+    {
+        sum *= f;
+        acc.x *= f;
+        acc.y *= f;
+        acc.z *= f;
+        acc.w *= f;
+    }
+    __device__ __forceinline__ void add(float l, const float4& y, float f)
+    {
+        sum = fmaf(l, f, sum);
+        acc.x = fmaf(y.x, f, acc.x);
+        acc.y = fmaf(y.y, f, acc.y);
+        acc.z = fmaf(y.z, f, acc.z);
+        acc.w = fmaf(y.w, f, acc.w);
+    }
+};
+
+// G neighbouring threads share a quad's parts (thread k takes parts k, k + G, ...), K parts' loads in flight each.
+template <typename C, int HD, int ROWS, int TILES, int G>
+__device__ __forceinline__ void merge_item(const PaArgs& a, const PaItem& g)
+{
+    constexpr int K = 4, QW = 32 / G;                 // quads of a warp
+    constexpr size_t kMl = PaPart<HD, ROWS>::kMl;
+    const float c = a.scale_log2;
+    const int lane = threadIdx.x & 31, part0 = lane / QW;
+    const int n = g.used * (HD / 4), stride = kPmThreads / G * gridDim.y;
+    for (int e0 = (blockIdx.y * (kPmThreads / 32) + (threadIdx.x >> 5)) * QW; e0 < n; e0 += stride) {
+        const int e = e0 + lane % QW;
+        const PmQuad q = pm_quad<HD, TILES>(g, min(e, n - 1));
+        PmSum p;
+        for (int k0 = part0; k0 < g.parts; k0 += K * G) {
+            float2 w[K];
+            float4 y[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const uint8_t* pt = pa_part<HD, ROWS, TILES>(a.parts, g.c0, g.c0 + min(k0 + k * G, g.parts - 1), q.tile);
+                w[k] = __ldcg(reinterpret_cast<const float2*>(pt + kMl) + q.row);
+                y[k] = __ldcg(reinterpret_cast<const float4*>(pt) + q.at);
+            }
+            float now = p.top;
+#pragma unroll
+            for (int k = 0; k < K; ++k) now = fmaxf(now, w[k].x);      // past the last part: the last one's again
+            p.scale(pa_weight(p.top, now, c));
+            p.top = now;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (k0 + k * G < g.parts) p.add(w[k].y, y[k], pa_weight(w[k].x, now, c));
+        }
+#pragma unroll
+        for (int o = QW; o < 32; o <<= 1) {
+            const float top = __shfl_xor_sync(0xffffffffu, p.top, o), sum = __shfl_xor_sync(0xffffffffu, p.sum, o);
+            float4 y;
+            y.x = __shfl_xor_sync(0xffffffffu, p.acc.x, o);
+            y.y = __shfl_xor_sync(0xffffffffu, p.acc.y, o);
+            y.z = __shfl_xor_sync(0xffffffffu, p.acc.z, o);
+            y.w = __shfl_xor_sync(0xffffffffu, p.acc.w, o);
+            const float now = fmaxf(p.top, top), f0 = pa_weight(p.top, now, c), f1 = pa_weight(top, now, c);
+            const bool low = !(lane & o);              // both sides add in the same order
+            PmSum r;
+            r.add(low ? p.sum : sum, low ? p.acc : y, low ? f0 : f1);
+            r.add(low ? sum : p.sum, low ? y : p.acc, low ? f1 : f0);
+            r.top = now;
+            p = r;
+        }
+        const int pr = g.p0 + q.tile * g.gap + q.row, tok = by_grp(a, pr), row = g.start + tok;
+        if (part0 > 0 || e >= n || row >= a.b.rows) continue;
+        const float inv = 1.f / p.sum;
+        uint2 w = make_uint2(pack2<C>(p.acc.x * inv, p.acc.y * inv), pack2<C>(p.acc.z * inv, p.acc.w * inv));
+        if (p.sum == 0.f) w = make_uint2(0, 0);
+        *reinterpret_cast<uint2*>(static_cast<C*>(a.out) + ((size_t)row * a.hq + g.h * a.grp + (pr - tok * a.grp)) * HD + q.quad * 4) = w;
+    }
+}
 
 template <typename C, int HD, int ROWS, int TILES>
 __device__ __forceinline__ void merge_item(const PaArgs& a, const PaItem& g)
 {
-    constexpr int E = 2, K = 4;
-    constexpr size_t kMl = PaPart<HD, ROWS>::kMl;
-    const float c = a.scale_log2;
-    const int n = g.used * (HD / 4), stride = kPmThreads * gridDim.y;
-    const int used0 = min(g.used, g.gap);
-    for (int e0 = blockIdx.y * kPmThreads + threadIdx.x; e0 < n; e0 += E * stride) {
-        int tile[E], at[E], row[E];                   // tile, quad index and row in the tile's part
-        float top[E], sum[E];
-        float4 acc[E];
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int e = min(e0 + i * stride, n - 1);
-            tile[i] = TILES > 1 && e >= used0 * (HD / 4) ? 1 : 0;
-            at[i] = e - tile[i] * used0 * (HD / 4);
-            row[i] = at[i] % (tile[i] ? g.used - used0 : used0);
-            top[i] = -INFINITY;
-            sum[i] = 0.f;
-            acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        for (int k0 = 0; k0 < g.parts; k0 += K) {
-            float2 w[E][K];
-            float4 y[E][K];
-#pragma unroll
-            for (int k = 0; k < K; ++k)
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const uint8_t* pt = pa_part<HD, ROWS, TILES>(a.parts, g.c0, g.c0 + min(k0 + k, g.parts - 1), tile[i]);
-                    w[i][k] = __ldcg(reinterpret_cast<const float2*>(pt + kMl) + row[i]);
-                    y[i][k] = __ldcg(reinterpret_cast<const float4*>(pt) + at[i]);
-                }
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                float now = top[i];
-#pragma unroll
-                for (int k = 0; k < K; ++k) now = fmaxf(now, w[i][k].x);      // the clamped ones are a part's own again
-                const float f0 = pa_weight(top[i], now, c);
-                top[i] = now;
-                sum[i] *= f0;
-                acc[i].x *= f0;
-                acc[i].y *= f0;
-                acc[i].z *= f0;
-                acc[i].w *= f0;
-#pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    if (k0 + k >= g.parts) continue;
-                    const float f = pa_weight(w[i][k].x, now, c);
-                    sum[i] = fmaf(w[i][k].y, f, sum[i]);
-                    acc[i].x = fmaf(y[i][k].x, f, acc[i].x);
-                    acc[i].y = fmaf(y[i][k].y, f, acc[i].y);
-                    acc[i].z = fmaf(y[i][k].z, f, acc[i].z);
-                    acc[i].w = fmaf(y[i][k].w, f, acc[i].w);
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int quad = at[i] / (tile[i] ? g.used - used0 : used0);
-            const int p = g.p0 + tile[i] * g.gap + row[i], tok = p / a.grp, r = g.start + tok;
-            if (e0 + i * stride >= n || r >= a.b.rows) continue;
-            const float inv = 1.f / sum[i];
-            uint2 w = make_uint2(pack2<C>(acc[i].x * inv, acc[i].y * inv), pack2<C>(acc[i].z * inv, acc[i].w * inv));
-            if (sum[i] == 0.f) w = make_uint2(0, 0);
-            *reinterpret_cast<uint2*>(static_cast<C*>(a.out) + ((size_t)r * a.hq + g.h * a.grp + (p - tok * a.grp)) * HD + quad * 4) = w;
-        }
-    }
+    if (g.parts <= 4) merge_item<C, HD, ROWS, TILES, 1>(a, g);
+    else merge_item<C, HD, ROWS, TILES, 4>(a, g);
 }
 
 template <typename C, int HD>
@@ -111,8 +145,7 @@ int pa_launch_merge(const PaArgs* tiles, const PaArgs* few, int ctas, cudaStream
 {
     const PaArgs none{};
     const PaArgs& a = tiles ? *tiles : *few;
-    // an item of few rows is one pass of a block or two
-    const dim3 grid(ctas, tiles ? kPmBlocks : 2, tiles && few ? 2 : 1);
+    const dim3 grid(ctas, tiles ? kPmBlocks : kPmFewBlocks, tiles && few ? 2 : 1);
     return a.b.dtype == EXL3_F16 ? launch_merge<__half>(tiles ? *tiles : none, few ? *few : none, a.b.head_dim, grid, s)
                                  : launch_merge<__nv_bfloat16>(tiles ? *tiles : none, few ? *few : none, a.b.head_dim, grid, s);
 }

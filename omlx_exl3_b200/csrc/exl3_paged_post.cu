@@ -175,7 +175,7 @@ int exl3_check_paged(const exl3_paged_desc* b)
     if (!b || !b->k_pages || !b->v_pages || !b->page_table || !b->cu_rows || !b->lens) return EXL3_E_NULL;
     if (b->seqs < 1 || b->rows < 0 || b->table_cols < 1 || b->num_pages < 1 || b->hkv < 1) return EXL3_E_SHAPE;
     if (b->page_size < 16 || (b->page_size & (b->page_size - 1))) return EXL3_E_SHAPE;
-    if ((long long)b->table_cols * b->page_size > 0x7fffffffll) return EXL3_E_SHAPE;
+    if ((long long)b->table_cols * b->page_size > (1ll << 30)) return EXL3_E_SHAPE;
     if (b->head_dim != 64 && b->head_dim != 128) return EXL3_E_SHAPE;
     if (b->dtype != EXL3_F16 && b->dtype != EXL3_BF16) return EXL3_E_DTYPE;
     if (!aligned(b->k_pages, 16) || !aligned(b->v_pages, 16) || !aligned(b->page_table, 4) || !aligned(b->cu_rows, 4) ||

@@ -33,6 +33,7 @@ struct PaArgs {
     uint32_t* status;
     float scale_log2;
     int hq, grp, span, item;
+    uint32_t grp_magic;                               // ceil(2^32 / grp): x / grp = umulhi(x, grp_magic) for x < 2^25 (0: grp is 1)
     int lo, hi;                                       // sequences of lo < rows * grp <= hi are this kernel's
 };
 
@@ -55,80 +56,84 @@ struct PaSeg {
     int c0, c1;                                       // the CTAs that share the item
 };
 
+__device__ __forceinline__ int by_grp(const PaArgs& a, int x) { return a.grp_magic ? (int)__umulhi((uint32_t)x, a.grp_magic) : x; }
+
 // The list is laid out in units with `item` more in front of every item (what its start and end cost beside its steps):
-// short contexts would otherwise pile up in one share.
+// short contexts would otherwise pile up in one share. A share is ceil(length / CTAs) units. All of it is 32-bit and nearly
+// free of divisions (the host has checked that the list is short enough): this runs before the first load of a call.
 struct PaSched {
     const PaArgs& a;
-    long long total, begin, until;                    // the list's length, the current item's place in it, this share's end
-    int ctas, s, h, t, j, cap;
+    int share, begin, until;                          // a share's length, the current item's place in the list, this share's end
+    int s, h, t, j, cap;
+    int rows, len;                                    // of sequence s
 
     __device__ __forceinline__ explicit PaSched(const PaArgs& args) : a(args) {}
 
-    __device__ __forceinline__ int rows_of(int q) const { return a.b.cu_rows[q + 1] - a.b.cu_rows[q]; }
-    __device__ __forceinline__ bool takes(int rows) const
-    {
-        const long long packed = (long long)rows * a.grp;
-        return rows > 0 && packed > a.lo && packed <= a.hi;
-    }
+    __device__ __forceinline__ bool takes(int r) const { return r > 0 && r * a.grp > a.lo && r * a.grp <= a.hi; }
     // Positions the last row of item i sees, 0 .. the page table's reach.
-    __device__ __forceinline__ int item_end(int rows, int len, int i) const
+    __device__ __forceinline__ int item_end(int r, int n, int i) const
     {
-        const int last = min(rows * a.grp, (i + 1) * a.span) - 1;
-        const long long e = (long long)len - rows + last / a.grp + 1;
-        return (int)max(0ll, min(e, (long long)cap));
+        const int e = n - r + by_grp(a, min(r * a.grp, (i + 1) * a.span) - 1) + 1;
+        return max(0, min(e, cap));
     }
     __device__ __forceinline__ static int units_of(int end) { return max(1, (end + kPaStep - 1) / kPaStep); }
 
-    __device__ __forceinline__ long long seq_length(int q) const
+    // Rows and length of sequence q: a length that could not be one is taken as the nearest that could.
+    __device__ __forceinline__ void load(int q, int& r, int& n) const
     {
-        const int rows = q < a.b.seqs ? rows_of(q) : 0;
-        if (!takes(rows)) return 0;
-        const int len = a.b.lens[q];
-        long long n = 0;
-        for (int i = 0; i * a.span < rows * a.grp; ++i) n += units_of(item_end(rows, len, i)) + a.item;
-        return n * a.b.hkv;
+        r = a.b.cu_rows[q + 1] - a.b.cu_rows[q];
+        r = max(0, min(r, a.b.rows));
+        n = max(0, min(a.b.lens[q], cap + a.b.rows));
+    }
+
+    // Length of sequence q in the list, for one kv head.
+    __device__ __forceinline__ int head_length(int q) const
+    {
+        if (q >= a.b.seqs) return 0;
+        int r, n, sum = 0;
+        load(q, r, n);
+        if (!takes(r)) return 0;
+        for (int i = 0; i * a.span < r * a.grp; ++i) sum += units_of(item_end(r, n, i)) + a.item;
+        return sum;
     }
 
     // All lanes of the warp. This CTA's share of the list, and where it starts.
     __device__ __forceinline__ void start(int cta, int grid, int lane)
     {
         cap = a.b.table_cols * a.b.page_size;
-        long long first = 0;                          // this lane's part of the first 32 sequences
-        total = 0;
+        int first = 0, total = 0;                     // first: this lane's part of the first 32 sequences
         for (int q0 = 0; q0 < a.b.seqs; q0 += 32) {
-            long long n = seq_length(q0 + lane);
+            const int n = head_length(q0 + lane);
             if (q0 == 0) first = n;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-            total += n;
+            total += __reduce_add_sync(0xffffffffu, n) * a.b.hkv;
         }
         s = h = t = j = 0;
         begin = until = 0;
-        ctas = (int)min((long long)grid, total);
-        if (cta >= ctas) return;
-        const long long u = total * cta / ctas;
-        until = total * (cta + 1) / ctas;
-        long long before = 0, at = 0;
+        share = (total + grid - 1) / grid;
+        const int u = cta * share;
+        if (u >= total) return;
+        until = min(total, u + share);
+        int before = 0, at = 0;
         for (int q0 = 0; q0 < a.b.seqs; q0 += 32) {
-            const long long n = q0 == 0 ? first : seq_length(q0 + lane);
-            long long sum = n;                        // inclusive prefix
+            const int n = q0 == 0 ? first : head_length(q0 + lane);
+            int sum = n;                              // inclusive prefix
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+                const int v = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += v;
             }
-            const int k = __popc(__ballot_sync(0xffffffffu, before + sum <= u));
+            const int k = __popc(__ballot_sync(0xffffffffu, before + sum * a.b.hkv <= u));
             if (k < 32) {
+                const int per = __shfl_sync(0xffffffffu, n, k);
                 s = q0 + k;
-                at = u - before - (__shfl_sync(0xffffffffu, sum, k) - __shfl_sync(0xffffffffu, n, k));
-                const long long per = __shfl_sync(0xffffffffu, n, k) / a.b.hkv;
-                h = (int)(at / per);
+                at = u - before - (__shfl_sync(0xffffffffu, sum, k) - per) * a.b.hkv;
+                h = at / per;
                 at -= per * h;
                 break;
             }
-            before += __shfl_sync(0xffffffffu, sum, 31);
+            before += __shfl_sync(0xffffffffu, sum, 31) * a.b.hkv;
         }
-        const int rows = rows_of(s), len = a.b.lens[s];
+        load(s, rows, len);
         for (;;) {
             const int n = units_of(item_end(rows, len, t)) + a.item;
             if (at < n) break;
@@ -136,29 +141,28 @@ struct PaSched {
             ++t;
         }
         begin = u - at;
-        j = max(0, (int)at - a.item);                 // at < n: one of the item's units
+        j = max(0, at - a.item);                      // at < n: one of the item's units
     }
-
-    __device__ __forceinline__ int cta_of(long long place) const { return (int)(((place + 1) * ctas - 1) / total); }
 
     // The next segment of this CTA's share; false when it is done.
     __device__ __forceinline__ bool next(PaSeg& g)
     {
         if (begin + a.item >= until) return false;    // no unit of the current item is in the share
-        const int rows = rows_of(s), len = a.b.lens[s];
         g.s = s;
         g.h = h;
         g.p0 = t * a.span;
         g.start = a.b.cu_rows[s];
         g.rows = rows;
-        g.ctx = (int)max(-(1ll << 30), (long long)len - rows);
+        g.ctx = len - rows;
         g.end = item_end(rows, len, t);
         g.units = units_of(g.end);
         g.j0 = j;
-        g.j1 = (int)min((long long)g.units, until - begin - a.item);
-        const bool cut = j > 0 || g.j1 < g.units;
-        g.c0 = cut ? cta_of(begin + a.item) : 0;
-        g.c1 = cut ? cta_of(begin + a.item + g.units - 1) : 0;
+        g.j1 = min(g.units, until - begin - a.item);
+        g.c0 = g.c1 = 0;
+        if (j > 0 || g.j1 < g.units) {
+            g.c0 = (begin + a.item) / share;
+            g.c1 = (begin + a.item + g.units - 1) / share;
+        }
         j = 0;
         begin += a.item + g.units;
         if (begin < until) {
@@ -168,8 +172,8 @@ struct PaSched {
                 t = 0;
                 if (++h == a.b.hkv) {
                     h = 0;
-                    do ++s;
-                    while (s < a.b.seqs - 1 && !takes(rows_of(s)));
+                    do load(++s, rows, len);
+                    while (s < a.b.seqs - 1 && !takes(rows));
                 }
             }
         }
@@ -213,6 +217,14 @@ __device__ __forceinline__ void pa_record(const PaArgs& a, bool any, const PaSeg
         it.gap = gap;
     }
     a.items[blockIdx.x] = it;
+}
+
+// Whether every batch of these sizes has a list that 32 bits hold (and rows that by_grp divides); items of `span` rows.
+inline bool pa_list_fits(const PaArgs& a, int span)
+{
+    const long long packed = (long long)a.b.rows * a.grp;
+    const long long steps = ((long long)a.b.table_cols * a.b.page_size + kPaStep - 1) / kPaStep + 8;
+    return packed < (1 << 25) && (packed / span + a.b.seqs) * a.b.hkv < 0x7fffffffll / steps;
 }
 
 // One launch over the sequences a.lo < rows * grp <= a.hi. Both set a.span and a.item.
