@@ -392,13 +392,14 @@ EXL3_API int exl3_paged_qkv_post(const exl3_paged_desc* batch, const void* q, co
 /*
  * Attention of the batch's rows over their sequences' pages: out[r, h] = softmax_j(scale * q[r, h] . K[j, h / g])
  * V[j, h / g] over positions j <= the row's own, g = hq / hkv. q and out (rows, hq, head_dim) in the
- * cache's dtype, 16-byte aligned; q's rows q_stride elements apart. fp32 scores and statistics. The
+ * cache's dtype, 16-byte aligned; q's rows q_stride elements apart. fp32 scores and statistics. max_rows: most
+ * rows of any sequence where the caller knows it, else 0; it saves a launch and changes no result. The
  * workspace (exl3_paged_attn_workspace bytes, 256-byte aligned, any contents) must not be shared by calls
  * that overlap.
  */
 EXL3_API int exl3_paged_attn_workspace(const exl3_paged_desc* batch, int hq, size_t* bytes);
 EXL3_API int exl3_paged_attn(const exl3_paged_desc* batch, const void* q, long long q_stride, int hq, float scale,
-                             void* out, void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
+                             int max_rows, void* out, void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
 
 /*
  * Verification of drafted tokens (speculative sampling; no counterpart in the reference, where oMLX's MTP

@@ -148,6 +148,13 @@ __device__ __forceinline__ void tc_commit_if(uint64_t* bar, uint32_t go)
         : "memory");
 }
 
+__device__ __forceinline__ void mbar_arrive_if(uint64_t* bar, uint32_t go)
+{
+    asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n @q mbarrier.arrive.shared::cta.b64 _, [%0];\n}\n" ::"r"(smem_addr(bar)),
+                 "r"(go)
+                 : "memory");
+}
+
 // Bounded wait of a whole warp, with one answer for all its lanes.
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, uint64_t limit_ns = 2000000000ull)
 {
@@ -436,6 +443,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         const uint32_t s_t = tmem + lanes + slot * kPaStep, o_t = tmem + lanes + 256 + slot * HD;
         const float c = a.scale_log2;
         uint32_t n_s = 0, n_o = 0;
+        const uint32_t leader = elect_one();
         // A wait that gave up only clears ok: the warps stay in step with each other, since they meet at barriers.
         while (sched.next(g)) {
             const Item im = item_of(g);
@@ -456,26 +464,34 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                 if (!idle) {
                     const int step = g.j0 + (dual ? i : 2 * i + slot);
                     float x[kPaStep];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) tc_ld32(s_t + q * 32, *reinterpret_cast<float(*)[32]>(x + q * 32));
-                    tc_wait_ld();
+                    // the second half of the row is on its way while the first is looked at
                     const int see = limit - step * kPaStep;
-                    if (__any_sync(0xffffffffu, see < kPaStep)) {
+                    const bool masked = __any_sync(0xffffffffu, see < kPaStep);
+                    float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+                    tm_ld32(s_t, x);
+                    tm_ld32(s_t + 32, x + 32);
+                    tc_wait_ld();
 #pragma unroll
-                        for (int q = 0; q < kPaStep; ++q) x[q] = q < see ? x[q] : -INFINITY;
-                    }
-                    float t0 = max3(x[0], x[1], x[2]), t1 = max3(x[3], x[4], x[5]);
-                    float t2 = max3(x[6], x[7], x[8]), t3 = max3(x[9], x[10], x[11]);
+                    for (int half = 0; half < 2; ++half) {
+                        if (half == 0) {
+                            tm_ld32(s_t + 64, x + 64);
+                            tm_ld32(s_t + 96, x + 96);
+                        } else {
+                            tc_wait_ld();
+                        }
+                        if (masked) {
 #pragma unroll
-                    for (int q = 12; q + 8 <= kPaStep; q += 8) {
-                        t0 = max3(t0, x[q], x[q + 1]);
-                        t1 = max3(t1, x[q + 2], x[q + 3]);
-                        t2 = max3(t2, x[q + 4], x[q + 5]);
-                        t3 = max3(t3, x[q + 6], x[q + 7]);
+                            for (int q = 64 * half; q < 64 * half + 64; ++q) x[q] = q < see ? x[q] : -INFINITY;
+                        }
+#pragma unroll
+                        for (int q = 64 * half; q < 64 * half + 64; q += 8) {
+                            t0 = max3(t0, x[q], x[q + 1]);
+                            t1 = max3(t1, x[q + 2], x[q + 3]);
+                            t2 = max3(t2, x[q + 4], x[q + 5]);
+                            t3 = max3(t3, x[q + 6], x[q + 7]);
+                        }
                     }
-                    t0 = max3(t0, x[kPaStep - 4], x[kPaStep - 3]);
-                    t1 = max3(t1, x[kPaStep - 2], x[kPaStep - 1]);
-                    const float top = max3(max3(t0, t1, t2), t3, t3);
+                    const float top = fmaxf(max3(t0, t1, t2), t3);
                     const bool grow = (top - m) * c > kPaSlack;        // false for a row that has seen nothing yet
                     if (__any_sync(0xffffffffu, grow)) {
                         const float f = grow ? pa_weight(m, top, c) : 1.f;
@@ -486,7 +502,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                             for (int q = 0; q < HD; q += 16) {
                                 float o[16];
                                 uint32_t w[16];
-                                tc_ld16(o_t + q, o);
+                                tm_ld16(o_t + q, o);
                                 tc_wait_ld();
 #pragma unroll
                                 for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * f);
@@ -522,7 +538,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                             tc_wait_st();
                             tc_fence_before();
                             __syncwarp();
-                            if (lane == 0) mbar_arrive(&p_full[2 * slot]);
+                            mbar_arrive_if(&p_full[2 * slot], leader);
                         }
                     }
                     float l0, l1, l2, l3;
@@ -533,10 +549,8 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    if (idle) mbar_arrive(&p_full[2 * slot]);
-                    mbar_arrive(&p_full[2 * slot + 1]);
-                }
+                if (idle) mbar_arrive_if(&p_full[2 * slot], leader);
+                mbar_arrive_if(&p_full[2 * slot + 1], leader);
             }
             if (mine > 0) {
                 if (ok && !pa_wait(&o_full[slot], n_o & 1)) ok = false;
@@ -573,7 +587,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                 if (ch == 0) inv = 1.f / l;
                 float o[32];
                 if (mine > 0) {
-                    tc_ld32(o_t + ch * 32, o);
+                    tm_ld32(o_t + ch * 32, o);
                     tc_wait_ld();
                     if (sends) {
 #pragma unroll
@@ -738,12 +752,12 @@ extern "C" int exl3_paged_attn_workspace(const exl3_paged_desc* batch, int hq, s
 }
 
 extern "C" int exl3_paged_attn(const exl3_paged_desc* batch, const void* q, long long q_stride, int hq, float scale,
-                               void* out, void* workspace, size_t workspace_bytes, uint32_t* status, void* stream)
+                               int max_rows, void* out, void* workspace, size_t workspace_bytes, uint32_t* status, void* stream)
 {
     if (int e = check_attn(batch, hq)) return e;
     if (batch->rows == 0) return EXL3_OK;
     if (!q || !out || !status || !workspace) return EXL3_E_NULL;
-    if (q_stride < (long long)hq * batch->head_dim || !(scale > 0.f)) return EXL3_E_SHAPE;
+    if (q_stride < (long long)hq * batch->head_dim || !(scale > 0.f) || max_rows < 0) return EXL3_E_SHAPE;
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(status, 4) || !aligned(workspace, 256) || q_stride % 8)
         return EXL3_E_ALIGN;
     if (int e = check_device()) return e;
@@ -760,21 +774,27 @@ extern "C" int exl3_paged_attn(const exl3_paged_desc* batch, const void* q, long
     a.grp = hq / batch->hkv;
     a.grp_magic = a.grp == 1 ? 0u : (uint32_t)(((1ull << 32) + a.grp - 1) / a.grp);
     if (!pa_list_fits(a, 8)) return EXL3_E_SHAPE;
-    // Which kernel takes a sequence goes by its packed rows, which only the device knows, unless there is one sequence. A
-    // batch with a row per sequence at most is taken for single tokens: one launch, right whatever the rows are.
+    // Which kernel takes a sequence goes by its packed rows, which only the device knows: the host launches what they may need,
+    // from their average and what it knows of the most. A 128-row tile costs the same however empty it is, but more at the
+    // start; 16 rows at a time read the keys and values once per 16. Measured, us with sequences of up to 32 / up to 64
+    // packed rows on the latter: 9 of 1 to 8 rows (4200 positions, group 5) 28.3 / 18.2; 16 of 8 rows over 2000 (40 each)
+    // 49.2 / 67.5; 64 of 4 rows (20 each) 38.8, and 51.0 on tiles. A batch with a row per sequence at most is taken for
+    // single tokens: one launch, right whatever the rows are.
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool few_only = a.grp <= kPaFew && (batch->seqs == 1 ? (long long)batch->rows * a.grp <= kPaFew
-                                                               : batch->rows <= batch->seqs);
-    const bool tiles_only = !few_only && (batch->seqs == 1 || a.grp > kPaFew);
+    const long long packed = (long long)batch->rows * a.grp;
+    const int hi = packed <= 32ll * batch->seqs ? 64 : 32;
+    const long long most = max_rows > 0 && max_rows < batch->rows ? (long long)max_rows * a.grp : packed;
+    const bool few_only = most <= hi || (batch->rows <= batch->seqs && a.grp <= hi);
+    const bool tiles_only = !few_only && (batch->seqs == 1 || a.grp > hi);
     uint8_t* base = static_cast<uint8_t*>(workspace);
     PaArgs few = a, tiles = a;
     few.items = reinterpret_cast<PaItem*>(base + w.few_items);
     few.parts = base + w.few_parts;
     few.lo = 0;
-    few.hi = few_only ? 0x7fffffff : kPaFew;
+    few.hi = few_only ? 0x7fffffff : hi;
     tiles.items = reinterpret_cast<PaItem*>(base);
     tiles.parts = base + w.tile_parts;
-    tiles.lo = tiles_only ? 0 : kPaFew;
+    tiles.lo = tiles_only ? 0 : hi;
     tiles.hi = 0x7fffffff;
     if (!tiles_only)
         if (int e = pa_launch_few(few, s)) return e;

@@ -186,11 +186,12 @@ def _attn_workspace_bytes(b: PagedDesc, hq: int, dev: int) -> int:
 
 def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                cu_rows: torch.Tensor, lens: torch.Tensor, scale: float | None = None,
-               out: torch.Tensor | None = None) -> torch.Tensor:
+               out: torch.Tensor | None = None, max_rows: int = 0) -> torch.Tensor:
     """Attention of q (rows, hq, head_dim) over the pages: row r sees positions up to its own of its sequence
     (grouped heads: head h reads kv head h // (hq // hkv)). scale defaults to 1 / sqrt(head_dim). Returns
     (rows, hq, head_dim) in q's dtype, which is the cache's. Rows at negative positions give zeros; what lies behind a
-    sequence's end in its pages is never used.
+    sequence's end in its pages is never used. max_rows, the most rows of any sequence where the caller knows it, may save
+    a launch; it changes no result.
     """
     if q.dim() != 3:
         raise ValueError("q must be (rows, hq, head_dim)")
@@ -198,7 +199,7 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     b, dev = _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows)
     if _get_device() != dev:                      # the kernels launch on the current device
         with torch.cuda.device(dev):
-            return paged_attn(q, k_pages, v_pages, page_table, cu_rows, lens, scale, out)
+            return paged_attn(q, k_pages, v_pages, page_table, cu_rows, lens, scale, out, max_rows)
     if q.dtype is not k_pages.dtype:
         raise TypeError("q must have the cache's dtype")
     if hd != b.head_dim or q.get_device() != dev:
@@ -221,7 +222,7 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
         return out
     stream = stream_ptr(dev)
     ws = _workspace(dev, stream, _attn_workspace_bytes(b, hq, dev))
-    status = lib().exl3_paged_attn(b, q.data_ptr(), s0, hq, scale, out.data_ptr(), ws.data_ptr(), ws.numel(),
+    status = lib().exl3_paged_attn(b, q.data_ptr(), s0, hq, scale, max_rows, out.data_ptr(), ws.data_ptr(), ws.numel(),
                                    _status_word(dev), stream)
     if status:
         check(status, "exl3_paged_attn")

@@ -118,7 +118,7 @@ def test_descriptor_refusals(kw, status):
     L, n = _lib.lib(), ctypes.c_size_t()
     assert L.exl3_paged_attn_workspace(_desc(**kw), 4, ctypes.byref(n)) == status
     P = 1 << 20
-    assert L.exl3_paged_attn(_desc(**kw), P, 512, 4, 1.0, P, P, 1 << 30, P, None) == status
+    assert L.exl3_paged_attn(_desc(**kw), P, 512, 4, 1.0, 0, P, P, 1 << 30, P, None) == status
     assert L.exl3_paged_qkv_post(_desc(**kw), P, P, P, 512, 256, 256, 0, 4, None, None, 1e-6, P, P, 10, 64, P, P, None) == status
 
 
@@ -130,10 +130,10 @@ def test_call_refusals():
     for hq in (0, 3, 2 * 129):
         assert L.exl3_paged_attn_workspace(d, hq, ctypes.byref(n)) == -1
 
-    def attn(q=P, qs=512, hq=4, scale=1.0, out=P, ws=P, wsb=1 << 30, st=P, b=d):
-        return L.exl3_paged_attn(b, q, qs, hq, scale, out, ws, wsb, st, None)
+    def attn(q=P, qs=512, hq=4, scale=1.0, most=0, out=P, ws=P, wsb=1 << 30, st=P, b=d):
+        return L.exl3_paged_attn(b, q, qs, hq, scale, most, out, ws, wsb, st, None)
     assert attn(q=None) == attn(out=None) == attn(st=None) == -6
-    assert attn(qs=511) == attn(scale=0.0) == attn(scale=float("nan")) == attn(hq=5) == -1
+    assert attn(most=-1) == attn(qs=511) == attn(scale=0.0) == attn(scale=float("nan")) == attn(hq=5) == -1
     assert attn(q=P + 2) == attn(out=P + 8) == attn(qs=513) == -5
     assert attn(b=_desc(rows=0)) == 0                                  # nothing to do
 

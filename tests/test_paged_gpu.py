@@ -129,6 +129,15 @@ def test_attn_scale_out_and_repeat(cuda):
         assert torch.equal(_attn(q, b, scale=0.25), out)
 
 
+@pytest.mark.parametrize("max_rows", [1, 4, 30, 1000])
+def test_attn_most_rows_changes_no_result(cuda, max_rows):
+    """Known, unknown or wrong: every row is computed, within the bound."""
+    rows, lens = [30, 1, 4], [700, 260, 9]
+    b = make_batch(rows, lens, 2, 128, 16, torch.float16, cuda, seed=40)
+    q = torch.randn((35, 10, 128), generator=torch.Generator().manual_seed(40)).half().to(cuda)
+    _check_attn(_attn(q, b, max_rows=max_rows), q, b, torch.float16)
+
+
 def test_attn_streams_do_not_share_scratch(cuda):
     """Calls on several streams at once, each against its own result alone."""
     sets = []
