@@ -25,6 +25,7 @@ from torch import nn
 from .kernels import (MAX_GEMV_ROWS, TrellisGemvPlan, add_norm_rot, argmax, attn_fits, attn_rot, norm_rot, qkv_post,
                       rot, swiglu_rot)
 from .linear import EXL3Linear
+from .paged import PagedBatch, PagedKVCache, paged_attn, paged_qkv_post
 
 # Up to this MLP width (per rank) the decode step's down_proj GEMV computes SwiGLU and its input rotation
 # itself (TrellisGemvPlan.swiglu_call), one launch less. Every CTA rotates the k blocks its units read, so
@@ -197,6 +198,15 @@ class Attention(nn.Module):
         o = o[0].transpose(0, 1).reshape(rows, self.hq * hd).to(x.dtype)
         return self.tp.all_reduce(self.o_proj(o))
 
+    def forward_paged(self, x: torch.Tensor, layer: int, cache: PagedKVCache, batch: PagedBatch, cos, sin) -> torch.Tensor:
+        """The same over a paged cache: the rows of every sequence of the batch, appended and attended to in two calls. Norm and
+        rotation are rounded once, to the cache's dtype (forward rounds to the model's in between)."""
+        kp, vp = cache.k[layer], cache.v[layer]
+        q = paged_qkv_post(self.q_proj(x), self.k_proj(x), self.v_proj(x), self.q_norm.weight, self.k_norm.weight,
+                           self.q_norm.eps, cos, sin, kp, vp, *batch.tables)
+        o = paged_attn(q, kp, vp, *batch.tables, max_rows=batch.max_rows)
+        return self.tp.all_reduce(self.o_proj(o.reshape(x.shape[0], -1).to(x.dtype)))
+
 
 class MLP(nn.Module):
     def __init__(self, cfg: ModelConfig, tp: TP, bits: dict, device):
@@ -222,6 +232,10 @@ class DecoderLayer(nn.Module):
 
     def forward(self, x, layer, cache, pos, cos, sin):
         h = x + self.self_attn(self.input_layernorm(x), layer, cache, pos, cos, sin)
+        return h + self.tp.all_reduce(self.mlp(self.post_attention_layernorm(h)))
+
+    def forward_paged(self, x, layer, cache, batch, cos, sin):
+        h = x + self.self_attn.forward_paged(self.input_layernorm(x), layer, cache, batch, cos, sin)
         return h + self.tp.all_reduce(self.mlp(self.post_attention_layernorm(h)))
 
 
@@ -361,6 +375,22 @@ class Qwen3EXL3(nn.Module):
         dev = device or self.rope_cos.device
         return KVCache(self.cfg.num_hidden_layers, self.cfg.num_key_value_heads // self.tp.size, max_len,
                        self.cfg.head_dim, dev)
+
+    def make_paged_cache(self, num_pages: int, page_size: int = 64, device=None, dtype=torch.float16) -> PagedKVCache:
+        """Pages for this rank's kv heads in every layer (forward_paged)."""
+        return PagedKVCache(self.cfg.num_hidden_layers, self.cfg.num_key_value_heads // self.tp.size, self.cfg.head_dim,
+                            num_pages, page_size, device or self.rope_cos.device, dtype)
+
+    @torch.no_grad()
+    def forward_paged(self, tokens: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
+                      rows: torch.Tensor | None = None) -> torch.Tensor:
+        """The rows of several sequences at once (prompt chunks, decoded tokens, drafts): tokens (batch.total_rows) in the
+        batch's row order, appended to their pages. Returns this rank's logits of `rows` (all rows where None)."""
+        x = self.model.embed_tokens(tokens)
+        for i, layer in enumerate(self.model.layers):
+            x = layer.forward_paged(x, i, cache, batch, self.rope_cos, self.rope_sin)
+        h = self.model.norm(x if rows is None else x.index_select(0, rows))
+        return self.lm_head(h) if self.lm_head is not None else h
 
     def hidden(self, tokens: torch.Tensor, cache: KVCache, pos: torch.Tensor) -> torch.Tensor:
         x = self.model.embed_tokens(tokens)

@@ -67,22 +67,21 @@ def check_paged_status(device: torch.device | None = None) -> None:
 _F16, _BF16, _I32, _F32 = torch.float16, torch.bfloat16, torch.int32, torch.float32
 
 
-def _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows: int) -> tuple[PagedDesc, int]:
-    """Checked descriptor of the batch (what can be checked without reading device memory) and its device."""
+def _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows: int) -> tuple:
+    """Checked descriptor of the batch (what can be checked without reading device memory), its device, hkv and head_dim."""
     dt = k_pages.dtype
     if (dt is not _F16 and dt is not _BF16) or v_pages.dtype is not dt:
         raise TypeError("k_pages and v_pages must both be fp16 or both bf16")
-    if page_table.dtype is not _I32 or cu_rows.dtype is not _I32 or lens.dtype is not _I32:
+    if not (page_table.dtype is cu_rows.dtype is lens.dtype is _I32):
         raise TypeError("page_table, cu_rows and lens must be int32")
     dev = k_pages.get_device()
     if dev < 0:
         raise ValueError("EXL3 kernels take CUDA tensors")
     if not (v_pages.get_device() == page_table.get_device() == cu_rows.get_device() == lens.get_device() == dev):
         raise ValueError("the pages and the batch's tables must be on one device")
-    shape = k_pages.shape
+    shape, table = k_pages.shape, page_table.shape
     if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError("pages must be (num_pages, hkv, page_size, head_dim), K and V alike")
-    table = page_table.shape
     if len(table) != 2 or cu_rows.dim() != 1 or lens.dim() != 1:
         raise ValueError("page_table is 2-d, cu_rows and lens 1-d")
     seqs, cols = table
@@ -94,17 +93,27 @@ def _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows: int) -> tuple
         raise ValueError("page_table, cu_rows and lens must be contiguous")
     num, hkv, ps, hd = shape
     return PagedDesc(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), cu_rows.data_ptr(), lens.data_ptr(),
-                     seqs, rows, cols, num, ps, hkv, hd, 0 if dt is _F16 else 1), dev
+                     seqs, rows, cols, num, ps, hkv, hd, 0 if dt is _F16 else 1), dev, hkv, hd
 
 
-def _row_stride(x: torch.Tensor, width: int, name: str) -> int:
+def _row_stride(x: torch.Tensor, rows: int, width: int, name: str) -> int:
     """Row stride in elements of a (rows, width) view with contiguous rows."""
-    if x.dim() != 2 or x.shape[1] != width:
-        raise ValueError(f"{name} must be (rows, {width})")
+    if x.shape != (rows, width):
+        raise ValueError(f"{name} must be ({rows}, {width})")
     s0, s1 = x.stride()
-    if s1 != 1 or (s0 < width and x.shape[0] > 1):
+    if s1 == 1 and s0 >= width:
+        return s0
+    if rows > 1 or s1 != 1 and width > 1:
         raise ValueError(f"{name} needs contiguous, non-overlapping rows")
-    return s0 if s0 > width else width
+    return width
+
+
+def _weight(w: torch.Tensor, dt: torch.dtype, hd: int, dev: int) -> int:
+    if w.dtype is not dt:
+        raise TypeError("norm weights must have q's dtype")
+    if w.numel() != hd or not w.is_contiguous() or w.get_device() != dev:
+        raise ValueError("norm weights must be contiguous (head_dim) on the pages' device")
+    return w.data_ptr()
 
 
 def paged_qkv_post(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm_w: torch.Tensor | None,
@@ -119,42 +128,33 @@ def paged_qkv_post(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm_w: 
     are rotated. Computed in fp32 and rounded once, to the cache's dtype. Two live rows of a call must not share a position.
     """
     rows, width = q.shape
-    b, dev = _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows)
+    b, dev, hkv, hd = _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows)
     if _get_device() != dev:                      # the kernels launch on the current device
         with torch.cuda.device(dev):
             return paged_qkv_post(q, k, v, q_norm_w, k_norm_w, eps, cos, sin, k_pages, v_pages, page_table, cu_rows, lens, q_out)
-    hd, hkv, dt = b.head_dim, b.hkv, q.dtype
+    dt, kv_dt, nk = q.dtype, k_pages.dtype, hkv * hd
     if (dt is not _F16 and dt is not _BF16) or k.dtype is not dt or v.dtype is not dt:
         raise TypeError("q, k and v must all be fp16 or all bf16")
-    if k.shape[0] != rows or v.shape[0] != rows:
-        raise ValueError("q, k and v must have the same rows")
-    if width == 0 or width % (hkv * hd):
+    if width == 0 or width % nk:
         raise ValueError("q's width must be a multiple of hkv * head_dim")
     hq = width // hd
-    sq, sk, sv = _row_stride(q, width, "q"), _row_stride(k, hkv * hd, "k"), _row_stride(v, hkv * hd, "v")
-    if cos.dtype is not _F32 or sin.dtype is not _F32:
+    sq, sk, sv = _row_stride(q, rows, width, "q"), _row_stride(k, rows, nk, "k"), _row_stride(v, rows, nk, "v")
+    if not (cos.dtype is sin.dtype is _F32):
         raise TypeError("cos and sin must be fp32")
-    if cos.dim() != 2 or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()):
+    rope = cos.shape
+    if len(rope) != 2 or sin.shape != rope or not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError("cos and sin must be contiguous (positions, rotated / 2)")
     if not (q.get_device() == k.get_device() == v.get_device() == cos.get_device() == sin.get_device() == dev):
         raise ValueError("all tensors must be on one device")
-    weights = [None, None]
-    for i, w in enumerate((q_norm_w, k_norm_w)):
-        if w is not None:
-            if w.dtype is not dt:
-                raise TypeError("norm weights must have q's dtype")
-            if w.numel() != hd or not w.is_contiguous() or w.get_device() != dev:
-                raise ValueError("norm weights must be contiguous (head_dim) on the pages' device")
-            weights[i] = w.data_ptr()
+    wq = None if q_norm_w is None else _weight(q_norm_w, dt, hd, dev)
+    wk = None if k_norm_w is None else _weight(k_norm_w, dt, hd, dev)
     if q_out is None:
-        q_out = torch.empty((rows, hq, hd), dtype=k_pages.dtype, device=k_pages.device)
-    elif (q_out.shape != (rows, hq, hd) or q_out.dtype is not k_pages.dtype or not q_out.is_contiguous()
-          or q_out.get_device() != dev):
+        q_out = q.new_empty((rows, hq, hd)) if kv_dt is dt else q.new_empty((rows, hq, hd), dtype=kv_dt)
+    elif q_out.shape != (rows, hq, hd) or q_out.dtype is not kv_dt or not q_out.is_contiguous() or q_out.get_device() != dev:
         raise ValueError("q_out must be contiguous (rows, hq, head_dim) in the cache's dtype")
-    n_rope, half = cos.shape
     status = lib().exl3_paged_qkv_post(b, q.data_ptr(), k.data_ptr(), v.data_ptr(), sq, sk, sv, 0 if dt is _F16 else 1, hq,
-                                       weights[0], weights[1], eps, cos.data_ptr(), sin.data_ptr(), n_rope, half,
-                                       q_out.data_ptr(), _status_word(dev), stream_ptr(dev))
+                                       wq, wk, eps, cos.data_ptr(), sin.data_ptr(), *rope, q_out.data_ptr(),
+                                       _status_word(dev), stream_ptr(dev))
     if status:
         check(status, "exl3_paged_qkv_post")
     return q_out
@@ -174,16 +174,6 @@ def _workspace(index: int, stream: int, nbytes: int) -> torch.Tensor:
 _attn_bytes: dict = {}
 
 
-def _attn_workspace_bytes(b: PagedDesc, hq: int, dev: int) -> int:
-    """Depends on the device and the head size alone."""
-    need = _attn_bytes.get((dev, b.head_dim))
-    if need is None:
-        size = ctypes.c_size_t()
-        check(lib().exl3_paged_attn_workspace(b, hq, ctypes.byref(size)), "exl3_paged_attn_workspace")
-        need = _attn_bytes[(dev, b.head_dim)] = size.value
-    return need
-
-
 def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                cu_rows: torch.Tensor, lens: torch.Tensor, scale: float | None = None,
                out: torch.Tensor | None = None, max_rows: int = 0) -> torch.Tensor:
@@ -196,15 +186,15 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     if q.dim() != 3:
         raise ValueError("q must be (rows, hq, head_dim)")
     rows, hq, hd = q.shape
-    b, dev = _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows)
+    b, dev, hkv, head_dim = _descriptor(k_pages, v_pages, page_table, cu_rows, lens, rows)
     if _get_device() != dev:                      # the kernels launch on the current device
         with torch.cuda.device(dev):
             return paged_attn(q, k_pages, v_pages, page_table, cu_rows, lens, scale, out, max_rows)
     if q.dtype is not k_pages.dtype:
         raise TypeError("q must have the cache's dtype")
-    if hd != b.head_dim or q.get_device() != dev:
+    if hd != head_dim or q.get_device() != dev:
         raise ValueError("q must be (rows, hq, head_dim) on the pages' device")
-    if hq < 1 or hq % b.hkv or hq // b.hkv > 128:
+    if hq < 1 or hq % hkv or hq // hkv > 128:
         raise ValueError("hq must be a multiple of hkv, at most 128 heads per kv head")
     if scale is None:
         scale = 1.0 / math.sqrt(hd)
@@ -215,15 +205,19 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
         q = q.contiguous()
         s0 = hq * hd
     if out is None:
-        out = torch.empty((rows, hq, hd), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != (rows, hq, hd) or out.dtype is not q.dtype or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError("out must be contiguous (rows, hq, head_dim) in q's dtype")
     if rows == 0:
         return out
     stream = stream_ptr(dev)
-    ws = _workspace(dev, stream, _attn_workspace_bytes(b, hq, dev))
-    status = lib().exl3_paged_attn(b, q.data_ptr(), s0, hq, scale, max_rows, out.data_ptr(), ws.data_ptr(), ws.numel(),
-                                   _status_word(dev), stream)
+    need = _attn_bytes.get((dev, hd))
+    if need is None:                              # depends on the device and the head size alone
+        size = ctypes.c_size_t()
+        check(lib().exl3_paged_attn_workspace(b, hq, size), "exl3_paged_attn_workspace")
+        need = _attn_bytes[(dev, hd)] = size.value
+    status = lib().exl3_paged_attn(b, q.data_ptr(), s0, hq, scale, max_rows, out.data_ptr(), _workspace(dev, stream, need).data_ptr(),
+                                   need, _status_word(dev), stream)
     if status:
         check(status, "exl3_paged_attn")
     return out

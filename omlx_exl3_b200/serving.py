@@ -1,0 +1,149 @@
+"""A small engine over the paged cache: many sequences, prompts in chunks, drafts verified on the GPU.
+
+The reference's scheduler (continuous batching, MTP drafting and verification) is oMLX's; PagedEngine is the least
+that runs the paged operators as a server does. One step is one batch: a chunk of the prompts that are not read yet, and for
+every other sequence its last token with the drafts that a proposer offers. Its logits go to verify_drafts, what was not
+accepted leaves the cache again, and the host reads one small tensor of tokens a step.
+
+    engine = PagedEngine(model, num_pages=4096)
+    engine.add("a", prompt_ids, max_new=200, temperature=0.7)
+    while engine.running:
+        for key, tokens in engine.step().items(): ...
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass, field
+
+import torch
+
+from .model import Qwen3EXL3
+from .paged import check_paged_status
+from .speculative import verify_drafts
+
+
+def lookup_drafts(tokens: list[int], most: int, longest: int = 3) -> list[int]:
+    """Drafts from the sequence's own text: what followed the last earlier occurrence of its final tokens (the longest
+    of up to `longest` that occurs), at most `most` of it."""
+    for n in range(min(longest, len(tokens) - 1), 0, -1):
+        tail = tokens[-n:]
+        for at in range(len(tokens) - n - 1, -1, -1):
+            if tokens[at:at + n] == tail:
+                return tokens[at + n:at + n + most]
+    return []
+
+
+@dataclass
+class _Sequence:
+    tokens: list[int]                   # prompt and what was generated
+    prompt: int                         # tokens of the prompt
+    max_new: int
+    temperature: float
+    stop: frozenset
+    new: list[int] = field(default_factory=list)
+
+
+class PagedEngine:
+    def __init__(self, model: Qwen3EXL3, num_pages: int, page_size: int = 64, chunk: int = 512, max_drafts: int = 4,
+                 propose=lookup_drafts, seed: int = 0, check_every: int = 64):
+        """chunk: prompt rows of a step; max_drafts: drafts of a sequence and step (0: none); propose(tokens, most) -> drafts."""
+        self.model, self.chunk, self.max_drafts, self.propose = model, chunk, max_drafts, propose
+        self.device = model.rope_cos.device
+        self.cache = model.make_paged_cache(num_pages, page_size)
+        self.check_every, self._unchecked = check_every, 0
+        self._gen = torch.Generator(device=self.device)
+        self._gen.manual_seed(seed)
+        self._seqs: dict = {}
+        self.drafted = self.accepted = 0
+
+    @property
+    def running(self) -> int:
+        return len(self._seqs)
+
+    def add(self, key, prompt: list[int], max_new: int, temperature: float = 0.0, stop=()) -> None:
+        """Queue a sequence; temperature 0 is greedy, `stop` are token ids that end it."""
+        if not prompt or max_new < 1 or temperature < 0:
+            raise ValueError("need a prompt, max_new of one or more and a temperature of zero or more")
+        if len(prompt) + max_new > self.model.cfg.max_position_embeddings:
+            raise ValueError(f"{len(prompt)} + {max_new} tokens exceed max_position_embeddings")
+        self.cache.add(key)
+        self._seqs[key] = _Sequence(list(prompt), len(prompt), max_new, float(temperature), frozenset(stop))
+
+    def _upload(self, values: list, dtype) -> torch.Tensor:
+        return torch.tensor(values, dtype=dtype).pin_memory().to(self.device, non_blocking=True)
+
+    def step(self) -> dict:
+        """One batch; returns the new tokens of the sequences that have some (finished ones leave the engine)."""
+        feeds, room = [], self.chunk
+        for key, s in self._seqs.items():
+            have = self.cache.length(key)
+            todo = s.prompt - have
+            if todo > 0:                                            # its prompt, as far as this step's chunk goes
+                n = min(todo, room)
+                room -= n
+                if n:
+                    feeds.append((key, s, s.tokens[have:have + n], [], n == todo))
+                continue
+            left = s.max_new - len(s.new)
+            drafts = self.propose(s.tokens, min(self.max_drafts, left - 1))[:left - 1] if self.max_drafts and left > 1 else []
+            feeds.append((key, s, [s.tokens[-1]] + drafts, drafts, True))
+        if not feeds:
+            return {}
+        lengths = {key: self.cache.length(key) for key, *_ in feeds}
+        batch = self.cache.extend([(key, len(rows)) for key, _, rows, _, _ in feeds])
+        tokens = self._upload([t for _, _, rows, _, _ in feeds for t in rows], torch.int64)
+        # rows whose logits are wanted: a decoding sequence's all, a finished prompt's last
+        judged = [(key, s, drafts) for key, s, _, drafts, wanted in feeds if wanted]
+        at, rows, cu = 0, [], [0]
+        for _, _, fed, drafts, wanted in feeds:
+            at += len(fed)
+            if wanted:
+                rows += range(at - len(drafts) - 1, at)
+                cu.append(len(rows))
+        logits = self.model.forward_paged(tokens, self.cache, batch, self._upload(rows, torch.int64) if rows else None)
+        out = {}
+        if judged:
+            out = self._verify(self.model.gather_logits(logits), judged, cu, lengths)
+        self._unchecked += 1
+        if self.check_every and self._unchecked >= self.check_every:
+            self._unchecked = 0
+            check_paged_status(self.device)
+        return out
+
+    def _verify(self, logits: torch.Tensor, judged: list, cu: list[int], lengths: dict) -> dict:
+        drafts = [t for _, _, d in judged for t in d]
+        most = max(len(d) for _, _, d in judged)
+        n, vocab = len(judged), logits.shape[1]
+        noise = torch.empty((n, vocab), device=self.device).exponential_(generator=self._gen).clamp_(min=1e-20)
+        u = torch.rand(len(drafts), device=self.device, generator=self._gen)
+        picked, count, _ = verify_drafts(logits, self._upload(drafts, torch.int64), self._upload(cu, torch.int32), u, noise, most,
+                                         temperature=self._upload([s.temperature for _, s, _ in judged], torch.float32))
+        picked = torch.cat([picked, count[:, None]], 1).tolist()    # the step's one wait for the GPU
+        out = {}
+        for (key, s, d), row in zip(judged, picked):
+            got = row[:row[-1]]
+            if got[-1] < 0:
+                raise RuntimeError(f"sequence {key!r}: the model gave no probabilities")
+            self.drafted += len(d)
+            self.accepted += len(got) - 1
+            if lengths[key] >= s.prompt:                            # its last token and the drafts that stand are cached
+                self.cache.truncate(key, lengths[key] + len(got))
+            end = next((i + 1 for i, t in enumerate(got) if t in s.stop), len(got))
+            got = got[:min(end, s.max_new - len(s.new))]
+            s.tokens += got
+            s.new += got
+            out[key] = got
+            if len(s.new) >= s.max_new or got[-1] in s.stop:
+                self.cache.release(key)
+                del self._seqs[key]
+        return out
+
+    def generate(self, prompts: list[list[int]], max_new: int, temperature: float = 0.0, stop=()) -> list[list[int]]:
+        """All of the prompts' continuations."""
+        done = {i: [] for i in range(len(prompts))}
+        for i, p in enumerate(prompts):
+            self.add(i, p, max_new, temperature, stop)
+        while self.running:
+            for i, got in self.step().items():
+                done[i] += got
+        check_paged_status(self.device)
+        return [done[i] for i in range(len(prompts))]

@@ -50,31 +50,30 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, cu_ro
         raise TypeError("u, noise and temperature must be fp32")
     if draft_tokens.shape != (drafts,) or u.shape != (drafts,):
         raise ValueError("draft_tokens and u must be (rows - seqs)")
-    if noise.shape != (seqs, n) or (temperature is not None and temperature.shape != (seqs,)):
-        raise ValueError("noise must be (seqs, n) and temperature (seqs)")
+    if temperature is not None and temperature.shape != (seqs,):
+        raise ValueError("temperature must be (seqs)")
     if not (cu_rows.is_contiguous() and draft_tokens.is_contiguous() and u.is_contiguous()
             and (temperature is None or temperature.is_contiguous())):
         raise ValueError("cu_rows, draft_tokens, u and temperature must be contiguous")
     if not (draft_tokens.get_device() == cu_rows.get_device() == u.get_device() == noise.get_device() == dev):
         raise ValueError("all tensors must be on one device")
-    ld, noise_ld = _row_stride(target_logits, n, "target_logits"), _row_stride(noise, n, "noise")
+    ld, noise_ld = _row_stride(target_logits, rows, n, "target_logits"), _row_stride(noise, seqs, n, "noise")
     draft_ptr, draft_ld, temp_ptr = None, n, None
     if draft_logits is not None:
         if draft_logits.dtype is not dt:
             raise TypeError("draft_logits must have target_logits' dtype")
-        if draft_logits.shape != (drafts, n) or draft_logits.get_device() != dev:
-            raise ValueError("draft_logits must be (rows - seqs, n) on target_logits' device")
-        draft_ld = _row_stride(draft_logits, n, "draft_logits")
+        if draft_logits.get_device() != dev:
+            raise ValueError("all tensors must be on one device")
+        draft_ld = _row_stride(draft_logits, drafts, n, "draft_logits")
         if drafts:
             draft_ptr = draft_logits.data_ptr()
     if temperature is not None:
         if temperature.get_device() != dev:
             raise ValueError("all tensors must be on one device")
         temp_ptr = temperature.data_ptr()
-    device = target_logits.device
-    tokens = torch.empty((seqs, max_drafts + 1), dtype=torch.int64, device=device)
-    count = torch.empty(seqs, dtype=_I32, device=device)
-    prob = torch.empty(drafts, dtype=_F32, device=device)
+    tokens = draft_tokens.new_empty((seqs, max_drafts + 1))
+    count = cu_rows.new_empty(seqs)
+    prob = u.new_empty(drafts)
     stream = stream_ptr(dev)
     size = ctypes.c_size_t()
     check(lib().exl3_verify_workspace(rows, seqs, n, size), "exl3_verify_workspace")
