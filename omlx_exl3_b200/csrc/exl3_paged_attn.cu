@@ -10,18 +10,21 @@
 // reads its row, keeps the running maximum and sum in registers, writes P back over S in the 16-bit type, and a
 // second tcgen05.mma adds P V to the accumulator in tensor memory.
 //
-// Roles of a CTA (one per SM, persistent): two softmax warpgroups, one warp that loads with TMA, one that
-// issues the MMAs. The tensor core alternates between two slots (S, P and O of their own) and works on one while the
-// other slot's softmax runs. In a two-tile item slot = tile; in a one-tile item the slots take alternate steps of the
-// same rows and are merged at its end. The accumulator is rescaled only when a row's maximum grows by more than 2^8
-// (P <= 256 is exact enough in either type, and the sum is fp32 of the unrounded p), by the softmax thread itself: S of
-// step j is only complete when P V of step j - 1 is, so nothing else touches the accumulator then.
+// Roles of a CTA (one per SM, persistent): two softmax warpgroups, one warp that loads with TMA, two that issue the
+// MMAs, one that cleans a tile's end. There are two slots (S, P and O of their own, a warpgroup and an issuing warp each). In a
+// two-tile item slot = tile; in a one-tile item the slots take alternate steps of the same rows and are merged at its
+// end. Within a slot a step goes by halves of 64 positions: while the softmax works on one half of S, the tensor core does
+// the other half's P V and then its S of the next step, in that order from one warp, so S may overwrite P. The
+// accumulator is rescaled only when a row's maximum grows by more than 2^8 (P <= 256 is exact enough in either type, and
+// the sum is fp32 of the unrounded p), by the softmax thread itself, once the P V issued last is complete.
 //
-// Split. All items' steps form one list (sequence, kv head, tile); each CTA takes an equal contiguous share of it,
-// computed by every warp from the device tables, so ragged batches and long contexts load all SMs evenly without
-// the host knowing a length. An item cut by a share's end leaves fp32 partials (m, l, O) in the workspace; the CTA that
-// arrives last on the item's counter merges them in CTA order: the result does not depend on who was last,
-// and no CTA waits for another.
+// Bound by the softmax (ex2: 128 x 128 of a tile step take 1024 cycles of the special function unit, as long as its 2 x 128^3
+// MMAs) and by what lies between: 1.06 PFLOP/s, 0.65 of a measured library GEMM, for 4096 rows over 8192 positions of
+// 40 / 8 heads of 128 in bf16 (486 us); an exponent polynomial on the FMA pipe for a quarter of the ex2 (553 against 507
+// us at that stage), four softmax warpgroups with a row's halves in two threads (589), and whole steps with an enforced
+// alternation of the slots' MMAs (497) were measured slower.
+//
+// Split: exl3_paged_sched.cuh; the parts of cut items are merged by exl3_paged_merge.cu.
 //
 // Positions are gathered by page: a step's tile is 128 / page_size TMA boxes per 64 columns (one for larger pages), pages
 // past the sequence's end are not read (zero fill), and what lies behind the end in its last page is masked in S and
@@ -42,10 +45,7 @@
 
 namespace exl3 {
 
-constexpr int kPaThreads = 384;                       // two softmax warpgroups; one with the load and the MMA warp
-// Registers of a softmax thread (a row's 128 scores stay in registers) and of the others: 2 x 200 + 104 = 3 x 168, what the
-// launch gives the three warpgroups together.
-constexpr int kPaSoftmaxRegs = 200, kPaOtherRegs = 104;
+constexpr int kPaThreads = 384;                       // two softmax warpgroups; one with the load, clean and MMA warps
 constexpr int kPaBarBytes = 512;
 constexpr uint64_t kPaExitNs = 100000000ull;          // wait for a CTA's own copies and MMAs before it exits
 
@@ -178,12 +178,12 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     uint64_t* empty = full + P::kStages;              // [stages] its MMAs are done
     uint64_t* q_full = empty + P::kStages;
     uint64_t* q_empty = q_full + 1;                   // the item's S are done and its merge buffer is read
-    uint64_t* s_full = q_empty + 1;                   // [2] S of the slot is complete (and the P V before it)
-    uint64_t* p_full = s_full + 2;                    // [2][2] half of P of the slot is written
-    uint64_t* v_dirty = p_full + 4;                   // the item's last V tile has landed and reaches past the sequence's end
+    uint64_t* s_full = q_empty + 1;                   // [2][2] half of S of the slot is complete (and that half's P V before it)
+    uint64_t* p_full = s_full + 4;                    // [2][2] half of P of the slot is written
+    uint64_t* pv_done = p_full + 4;                   // [2] P V of the first half of the slot's step is complete
+    uint64_t* v_dirty = pv_done + 2;                   // the item's last V tile has landed and reaches past the sequence's end
     uint64_t* v_clean = v_dirty + 1;                  // it is zero there
-    uint64_t* turn = v_clean + 1;                     // [2] the slot's MMAs of a step may be issued
-    uint64_t* o_full = turn + 2;                   // [2] the slot's accumulator is complete
+    uint64_t* o_full = v_clean + 1;                   // [2] the slot's accumulator is complete
     uint64_t* o_empty = o_full + 2;                   // [2] it has been read
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
 
@@ -198,10 +198,11 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         mbar_init(v_dirty, 1);
         mbar_init(v_clean, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1);
+            mbar_init(&s_full[2 * i], 1);
+            mbar_init(&s_full[2 * i + 1], 1);
+            mbar_init(&pv_done[i], 1);
             mbar_init(&p_full[2 * i], 4);
             mbar_init(&p_full[2 * i + 1], 4);
-            mbar_init(&turn[i], 1);
             mbar_init(&o_full[i], 1);
             mbar_init(&o_empty[i], 4);
         }
@@ -235,9 +236,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         i.ntok[1] = ntok - i.ntok[0];
         return i;
     };
-    if (warp >= 8) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPaOtherRegs));
-      if (warp == 8) {
+    if (warp == 8) {
         sched.start(blockIdx.x, gridDim.x, lane);
         // ---------------------------------------------------------------- loads
         const int ps = a.b.page_size;
@@ -299,7 +298,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         for (uint32_t i = it > (uint32_t)P::kStages ? it - P::kStages : 0; i < it; ++i)
             if (!pa_wait(&full[i % P::kStages], (i / P::kStages) & 1, kPaExitNs)) ok = false;
         if (n_seg > 0 && !pa_wait(q_full, (n_seg - 1) & 1, kPaExitNs)) ok = false;
-      } else if (warp == 10) {
+    } else if (warp == 10) {
         sched.start(blockIdx.x, gridDim.x, lane);
         // ---------------------------------------------------------------- V behind the sequence's end becomes zero
         uint32_t it = 0, n = 0;
@@ -317,14 +316,14 @@ __global__ void __launch_bounds__(kPaThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(v_clean);
         }
-      } else {
+    } else if (warp > 8) {
         sched.start(blockIdx.x, gridDim.x, lane);
         // ---------------------------------------------------------------- MMAs: warp 9 for slot 0, warp 11 for slot 1
         // Between the MMAs of a step lie waits and commits of some hundred cycles in the issuing warp; with a warp per slot
         // they pass while the other slot's MMAs run. Each whole warp runs this and one elected lane issues, so that operands
         // come from uniform registers. Both warps see every tile of the ring land and release it (the tiles of the other
         // slot at once), so neither can fall a round behind.
-        constexpr uint32_t idesc_s = pa_idesc<C>(kPaStep, false), idesc_o = pa_idesc<C>(HD, true);
+        constexpr uint32_t idesc_s = pa_idesc<C>(kPaStep / 2, false), idesc_o = pa_idesc<C>(HD, true);
         const int slot = warp == 11;
         const uint32_t leader = elect_one();
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
@@ -349,43 +348,31 @@ __global__ void __launch_bounds__(kPaThreads, 1)
             if (mine) commit(&empty[i]);
             else if (ok && lane == 0) mbar_arrive(&empty[i]);
         };
-        auto mma_s = [&](int tile, uint32_t stage) {
-            const uint64_t qd = q_desc + tile * (P::kTile >> 4), kd = k_desc + stage * (P::kTile >> 4);
+        // S of 64 of a step's positions
+        auto mma_s = [&](int tile, uint32_t stage, int half) {
+            const uint64_t qd = q_desc + tile * (P::kTile >> 4), kd = k_desc + stage * (P::kTile >> 4) + half * (8192 >> 4);
 #pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk) {
                 const int off = ((kk / 4) * P::kPanel + (kk % 4) * 32) >> 4;
-                tc_mma_if(s_tm, qd + off, kd + off, idesc_s, kk > 0, leader & (uint32_t)ok);
+                tc_mma_if(s_tm + half * 64, qd + off, kd + off, idesc_s, kk > 0, leader & (uint32_t)ok);
             }
-            commit(&s_full[slot]);
+            commit(&s_full[2 * slot + half]);
         };
-        // Turns: the slots issue their steps' MMAs alternately. Left alone the two fall into step, both in softmax and then both
-        // at the tensor core (602 against 507 us for the 4096-row chunk over 8192 positions).
-        uint32_t n_turn = 0;
-        auto my_turn = [&]() {
-            if (slot == 1 || n_turn > 0) wait(&turn[slot], (n_turn - (slot == 0 ? 1 : 0)) & 1);
-            ++n_turn;
-        };
-        auto pass_turn = [&]() {
-            if (ok && lane == 0) mbar_arrive(&turn[slot ^ 1]);
-        };
-        // P V of a step; `first`: the slot's first of the item
-        auto mma_o = [&](uint32_t stage, bool first) {
-            if (first) {
+        // P V of half of a step; `first`: the slot's first of the item
+        auto mma_o = [&](uint32_t stage, int half, bool first) {
+            if (first && half == 0) {
                 if (n_o > 0) wait(&o_empty[slot], (n_o - 1) & 1);
                 ++n_o;
             }
+            wait(&p_full[2 * slot + half], n_p & 1);
+            tc_fence_after();
             const uint64_t vd = v_desc + stage * (P::kTile >> 4);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                wait(&p_full[2 * slot + half], n_p & 1);
-                if (half == 0) my_turn();
-                tc_fence_after();
-#pragma unroll
-                for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                    tc_mma_ts_if(o_tm, s_tm + kk * 8, vd + kk * (2048 >> 4), idesc_o, (first && kk == 0) ? 0u : 1u,
-                                 leader & (uint32_t)ok);
-            }
-            ++n_p;
+            for (int kk = 0; kk < 4; ++kk)
+                tc_mma_ts_if(o_tm, s_tm + half * 64 + kk * 8, vd + (4 * half + kk) * (2048 >> 4), idesc_o,
+                             (first && half == 0 && kk == 0) ? 0u : 1u, leader & (uint32_t)ok);
+            if (half == 0) commit(&pv_done[slot]);
+            else ++n_p;
         };
         while (ok && sched.next(g)) {
             wait(q_full, n_seg & 1);
@@ -399,7 +386,8 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                 const bool mine = dual || i == slot;
                 if (mine) {
                     tc_fence_after();
-                    mma_s(dual ? slot : 0, k);
+                    mma_s(dual ? slot : 0, k, 0);
+                    mma_s(dual ? slot : 0, k, 1);
                 }
                 release(k, mine);
             }
@@ -414,27 +402,23 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                     wait(v_clean, n_clean++ & 1);
                 }
                 if (mine) {
-                    mma_o(v, m < ahead);
-                    if (more) mma_s(dual ? slot : 0, k);
-                    else commit(&o_full[slot]);
-                    pass_turn();
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        mma_o(v, half, m < ahead);
+                        if (more) mma_s(dual ? slot : 0, k, half);
+                    }
+                    if (!more) commit(&o_full[slot]);
                 }
                 release(v, mine);
                 if (more) release(k, mine);
                 if (m + 1 + ahead == n) commit(q_empty);
-            }
-            if (!dual && n % 2 && slot == 1) {
-                my_turn();
-                pass_turn();
             }
         }
         // the MMAs' last reads and commits before the CTA's memory goes
         const uint32_t taken = ring * P::kStages + st;
         for (uint32_t i = taken > (uint32_t)P::kStages ? taken - P::kStages : 0; i < taken; ++i)
             if (!pa_wait(&empty[i % P::kStages], (i / P::kStages) & 1, kPaExitNs)) ok = false;
-      }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPaSoftmaxRegs));
         sched.start(blockIdx.x, gridDim.x, lane);
         // ---------------------------------------------------------------- softmax and epilogue
         const int slot = warp >> 2, quarter = warp & 3;
@@ -458,99 +442,91 @@ __global__ void __launch_bounds__(kPaThreads, 1)
             const int n = g.j1 - g.j0;
             const int mine = dual ? n : (n + 1 - slot) / 2;
             for (int i = 0; i < mine; ++i) {
-                if (ok && !pa_wait(&s_full[slot], n_s & 1)) ok = false;
-                ++n_s;
-                tc_fence_after();
-                if (!idle) {
-                    const int step = g.j0 + (dual ? i : 2 * i + slot);
-                    float x[kPaStep];
-                    // the second half of the row is on its way while the first is looked at
-                    const int see = limit - step * kPaStep;
-                    const bool masked = __any_sync(0xffffffffu, see < kPaStep);
-                    float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
-                    tm_ld32(s_t, x);
-                    tm_ld32(s_t + 32, x + 32);
-                    tc_wait_ld();
+                const int step = g.j0 + (dual ? i : 2 * i + slot);
+                // 64 positions at a time: while one half of S is worked on here, the tensor core does the other half's
+                // P V and its S of the next step, so neither waits for the other's whole step
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    if (ok && !pa_wait(&s_full[2 * slot + half], n_s & 1)) ok = false;
+                    tc_fence_after();
+                    if (!idle) {
+                        const uint32_t x_t = s_t + half * 64;
+                        float x[64];
+                        tm_ld32(x_t, x);
+                        tm_ld32(x_t + 32, x + 32);
+                        tc_wait_ld();
+                        const int see = limit - step * kPaStep - half * 64;
+                        if (__any_sync(0xffffffffu, see < 64)) {
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        if (half == 0) {
-                            tm_ld32(s_t + 64, x + 64);
-                            tm_ld32(s_t + 96, x + 96);
-                        } else {
-                            tc_wait_ld();
+                            for (int q = 0; q < 64; ++q) x[q] = q < see ? x[q] : -INFINITY;
                         }
-                        if (masked) {
+                        float t0 = x[0], t1 = x[1], t2 = x[2], t3 = x[3];
 #pragma unroll
-                            for (int q = 64 * half; q < 64 * half + 64; ++q) x[q] = q < see ? x[q] : -INFINITY;
-                        }
-#pragma unroll
-                        for (int q = 64 * half; q < 64 * half + 64; q += 8) {
+                        for (int q = 4; q + 8 <= 64; q += 8) {
                             t0 = max3(t0, x[q], x[q + 1]);
                             t1 = max3(t1, x[q + 2], x[q + 3]);
                             t2 = max3(t2, x[q + 4], x[q + 5]);
                             t3 = max3(t3, x[q + 6], x[q + 7]);
                         }
-                    }
-                    const float top = fmaxf(max3(t0, t1, t2), t3);
-                    const bool grow = (top - m) * c > kPaSlack;        // false for a row that has seen nothing yet
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float f = grow ? pa_weight(m, top, c) : 1.f;
-                        if (grow) m = top;
-                        l *= f;
-                        if (i > 0) {
+                        t0 = max3(t0, x[60], x[61]);
+                        t1 = max3(t1, x[62], x[63]);
+                        const float top = fmaxf(max3(t0, t1, t2), t3);
+                        const bool grow = (top - m) * c > kPaSlack;    // false for a row that has seen nothing yet
+                        if (__any_sync(0xffffffffu, grow)) {
+                            const float f = grow ? pa_weight(m, top, c) : 1.f;
+                            if (grow) m = top;
+                            l *= f;
+                            if (i > 0 || half > 0) {
+                                // the P V issued last has to be complete: the other half's S follows it, or its own commit
+                                if (ok && !pa_wait(half ? &pv_done[slot] : &s_full[2 * slot + 1], n_s & 1)) ok = false;
+                                tc_fence_after();
 #pragma unroll 1
-                            for (int q = 0; q < HD; q += 16) {
-                                float o[16];
-                                uint32_t w[16];
-                                tm_ld16(o_t + q, o);
-                                tc_wait_ld();
+                                for (int q = 0; q < HD; q += 16) {
+                                    float o[16];
+                                    uint32_t w[16];
+                                    tm_ld16(o_t + q, o);
+                                    tc_wait_ld();
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * f);
-                                tc_st16(o_t + q, w);
+                                    for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * f);
+                                    tc_st16(o_t + q, w);
+                                }
+                                tc_wait_st();
                             }
-                            tc_wait_st();
                         }
-                    }
-                    const float mc = m == -INFINITY ? 0.f : m * c;
-                    const uint64_t c2 = f2(c, c), mc2 = f2(-mc, -mc);
-                    uint64_t l01 = f2(0.f, 0.f), l23 = l01;
-                    // p of the row, stored by 32 columns; the first half's P V runs beside the second half's exp
+                        const float mc = m == -INFINITY ? 0.f : m * c;
+                        const uint64_t c2 = f2(c, c), mc2 = f2(-mc, -mc);
+                        uint64_t l01 = f2(0.f, 0.f), l23 = l01;
 #pragma unroll
-                    for (int part = 0; part < 4; ++part) {
-                        uint32_t pk[16];
+                        for (int part = 0; part < 2; ++part) {
+                            uint32_t pk[16];
 #pragma unroll
-                        for (int q = 0; q < 32; q += 4) {
-                            const float* y = x + part * 32 + q;
-                            float e0, e1, e2, e3;
-                            f2_get(f2_fma(f2(y[0], y[1]), c2, mc2), e0, e1);
-                            f2_get(f2_fma(f2(y[2], y[3]), c2, mc2), e2, e3);
-                            e0 = ex2(e0);
-                            e1 = ex2(e1);
-                            e2 = ex2(e2);
-                            e3 = ex2(e3);
-                            l01 = f2_add(l01, f2(e0, e1));
-                            l23 = f2_add(l23, f2(e2, e3));
-                            pk[q / 2] = pack2<C>(e0, e1);
-                            pk[q / 2 + 1] = pack2<C>(e2, e3);
+                            for (int q = 0; q < 32; q += 4) {
+                                const float* y = x + part * 32 + q;
+                                float e0, e1, e2, e3;
+                                f2_get(f2_fma(f2(y[0], y[1]), c2, mc2), e0, e1);
+                                f2_get(f2_fma(f2(y[2], y[3]), c2, mc2), e2, e3);
+                                e0 = ex2(e0);
+                                e1 = ex2(e1);
+                                e2 = ex2(e2);
+                                e3 = ex2(e3);
+                                l01 = f2_add(l01, f2(e0, e1));
+                                l23 = f2_add(l23, f2(e2, e3));
+                                pk[q / 2] = pack2<C>(e0, e1);
+                                pk[q / 2 + 1] = pack2<C>(e2, e3);
+                            }
+                            tc_st16(x_t + part * 16, pk);
                         }
-                        tc_st16(s_t + part * 16, pk);
-                        if (part == 1) {
-                            tc_wait_st();
-                            tc_fence_before();
-                            __syncwarp();
-                            mbar_arrive_if(&p_full[2 * slot], leader);
-                        }
+                        float l0, l1, l2, l3;
+                        f2_get(l01, l0, l1);
+                        f2_get(l23, l2, l3);
+                        l += (l0 + l1) + (l2 + l3);
+                        tc_wait_st();
                     }
-                    float l0, l1, l2, l3;
-                    f2_get(l01, l0, l1);
-                    f2_get(l23, l2, l3);
-                    l += (l0 + l1) + (l2 + l3);
-                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    mbar_arrive_if(&p_full[2 * slot + half], leader);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (idle) mbar_arrive_if(&p_full[2 * slot], leader);
-                mbar_arrive_if(&p_full[2 * slot + 1], leader);
+                ++n_s;
             }
             if (mine > 0) {
                 if (ok && !pa_wait(&o_full[slot], n_o & 1)) ok = false;
