@@ -34,11 +34,11 @@ struct PfShape {
     static constexpr int kRow = HD * 2;               // bytes of a position
     static constexpr int kSlot = 2 * kPfSlice * kRow; // a slice's K and V
     static constexpr int kDepth = HD == 128 ? 3 : 6;  // slices of a warp's ring: 192 KB in all
-    static constexpr int kCols = NQ == 1 ? 64 : 32;   // columns merged at a time
+    static constexpr int kCols = NQ == 1 ? HD : 64;   // columns merged at a time: a quad for each of the CTA's threads
     static constexpr int kPad = kCols + 4;
     static constexpr int kMerge = kPfWarps * 8 * NQ * kPad * 4;
     static constexpr int kSmem = kPfWarps * kDepth * kSlot + kMerge;
-    static_assert(kSmem + 2048 <= 227 * 1024, "shared memory");
+    static_assert(kSmem + 2 * kPfWarps * 8 * NQ * 4 <= 227 * 1024, "shared memory");
 };
 
 template <typename C>
@@ -159,13 +159,9 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
     // ldmatrix addresses within a slot: K rows as they are, V transposed
     const int krow = lane & 15, kch = lane >> 4;
     const int vrow = (lane & 7) + ((lane >> 4) << 3), vch = (lane >> 3) & 1;
-    bool any = false;
-    while (sched.next(g)) {
-        any = true;
+    uint32_t qb[NQ][HD / 16][2];                      // Q^T fragments of segment g
+    auto load_q = [&]() {
         const int used = min(8 * NQ, g.rows * a.grp - g.p0);
-        // Q^T fragments, and what each of this lane's columns sees
-        uint32_t qb[NQ][HD / 16][2];
-        int lim[NQ][2], least = 0x7fffffff;
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
             const int p = g.p0 + 8 * t + gid, tok = by_grp(a, p), row = g.start + tok;
@@ -176,13 +172,22 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
                 qb[t][ks][0] = live ? *reinterpret_cast<const uint32_t*>(src + 16 * ks) : 0u;
                 qb[t][ks][1] = live ? *reinterpret_cast<const uint32_t*>(src + 16 * ks + 8) : 0u;
             }
+        }
+    };
+    bool more = sched.next(g);
+    const bool any = more;
+    if (more) load_q();
+    while (more) {
+        const int used = min(8 * NQ, g.rows * a.grp - g.p0);
+        int lim[NQ][2], least = 0x7fffffff;           // positions this lane's columns see
+#pragma unroll
+        for (int t = 0; t < NQ; ++t)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int q = 8 * t + 2 * tig + e;
                 lim[t][e] = q < used ? min(g.end, g.ctx + by_grp(a, g.p0 + q) + 1) : 0x7fffffff;
                 least = min(least, lim[t][e]);
             }
-        }
         if (lane == 0 && warp == 0 && g.ctx + by_grp(a, g.p0 + used - 1) >= sched.cap) atomicOr(a.status, kStatusPagedRange);
         float o[HD / 16][NQ][4] = {};
         float m[NQ][2], l[NQ][2];
@@ -257,6 +262,10 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
             }
         }
 
+        const PaSeg done = g;
+        more = sched.next(g);
+        if (more) load_q();                           // on their way while this segment is merged
+
         // ---- the warps' results, merged in warp order
 #pragma unroll
         for (int t = 0; t < NQ; ++t)
@@ -269,8 +278,8 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
                     wl[warp][8 * t + 2 * tig + e] = l[t][e];
                 }
             }
-        const bool whole = g.j0 == 0 && g.j1 == g.units;
-        uint8_t* part = pa_part<HD, kPaFew, 1>(a.parts, g.c0, blockIdx.x, 0);
+        const bool whole = done.j0 == 0 && done.j1 == done.units;
+        uint8_t* part = pa_part<HD, kPaFew, 1>(a.parts, done.c0, blockIdx.x, 0);
 #pragma unroll
         for (int c0 = 0; c0 < HD; c0 += S::kCols) {
 #pragma unroll
@@ -300,13 +309,13 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
                     acc.w += y.w * f;
                 }
                 if (whole) {
-                    const int p = g.p0 + r, tok = by_grp(a, p), row = g.start + tok;
+                    const int p = done.p0 + r, tok = by_grp(a, p), row = done.start + tok;
                     if (row < a.b.rows) {
                         const float inv = 1.f / sum;
                         uint2 w = make_uint2(pack2<C>(acc.x * inv, acc.y * inv), pack2<C>(acc.z * inv, acc.w * inv));
                         if (sum == 0.f) w = make_uint2(0, 0);
                         *reinterpret_cast<uint2*>(static_cast<C*>(a.out) +
-                                                  ((size_t)row * a.hq + g.h * a.grp + (p - tok * a.grp)) * HD + c0 + quad * 4) = w;
+                                                  ((size_t)row * a.hq + done.h * a.grp + (p - tok * a.grp)) * HD + c0 + quad * 4) = w;
                     }
                 } else {
                     __stcg(reinterpret_cast<float4*>(part) + (c0 / 4 + quad) * used + r, acc);
@@ -316,7 +325,7 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
             __syncthreads();
         }
     }
-    if (threadIdx.x == 0) pa_record(a, any, g, any ? min(8 * NQ, g.rows * a.grp - g.p0) : 0, 8 * NQ);
+    if (threadIdx.x == 0) pa_record(a, any, g, any ? min(8 * NQ, g.rows * a.grp - g.p0) : 0, 8 * NQ);   // g: the last segment
     cp_async_wait<0>();
 }
 
@@ -334,7 +343,7 @@ static int launch_few(const PaArgs& args, cudaStream_t s)
     }
     PaArgs a = args;
     a.span = 8 * NQ;
-    a.item = 4;
+    a.item = 2;
     const int ctas = device_sm_count();
     return launch_pdl(paged_few_kernel<C, HD, NQ>, dim3(ctas), dim3(32 * kPfWarps), PfShape<HD, NQ>::kSmem, s, a);
 }
