@@ -8,6 +8,8 @@ preconditions, kernels.py:269-270, :465; linear.py:60-61), CUDA failures raise R
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import threading
 
 import torch
@@ -131,6 +133,24 @@ def lib():
                     fn.argtypes = args
                 _lib = L
     return _lib
+
+
+_torch_calls = None
+
+
+def torch_calls():
+    """The native calls of the paged-serving operators (csrc/exl3_torch.cpp), built first if the source is newer."""
+    global _torch_calls
+    if _torch_calls is None:
+        lib()
+        with _lock:
+            if _torch_calls is None:
+                path = str(_build.build_binding())
+                loader = importlib.machinery.ExtensionFileLoader("_exl3_torch", path)
+                module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_exl3_torch", path, loader=loader))
+                loader.exec_module(module)
+                _torch_calls = module
+    return _torch_calls
 
 
 def check(status: int, what: str) -> None:

@@ -6,6 +6,9 @@ Every translation unit is compiled by nvcc with `-gencode arch=compute_100a,code
 architecture-specific target: tcgen05 / TMA instructions need the `a` variant), objects go to
 omlx_exl3_b200/_build/, and the shared library is linked in-tree next to this file so that it
 travels with the repository snapshot. nvcc cross-compiles; no GPU is needed to build.
+
+csrc/exl3_torch.cpp, the native argument checks of the paged-serving calls, is compiled by the host compiler against the
+installed torch into _exl3_torch.so beside it; it links libexl3b200.so.
 """
 from __future__ import annotations
 
@@ -13,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -22,6 +26,8 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 BUILD = PKG / "_build"
 LIB = PKG / "libexl3b200.so"
+BINDING_SRC = CSRC / "exl3_torch.cpp"
+BINDING = PKG / "_exl3_torch.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
@@ -48,6 +54,32 @@ def up_to_date() -> bool:
     return all(p.stat().st_mtime <= t for p in _deps())
 
 
+def binding_up_to_date() -> bool:
+    return BINDING.exists() and all(p.stat().st_mtime <= BINDING.stat().st_mtime
+                                    for p in [BINDING_SRC, *INCLUDE.glob("*.h")])
+
+
+def build_binding(force: bool = False) -> Path:
+    """Compile the torch binding (when its source changed); the library has to be there."""
+    if not force and binding_up_to_date():
+        return BINDING
+    import torch
+    troot = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent if shutil.which(nvcc()) else Path("/usr/local/cuda")
+    tmp = BINDING.with_suffix(f".so.{os.getpid()}.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", str(troot / "include"), "-isystem", str(troot / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_path("include"), f"-I{INCLUDE}",
+           str(BINDING_SRC), "-o", str(tmp), f"-L{PKG}", "-lexl3b200", f"-L{troot / 'lib'}", "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on {BINDING_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def _compile(src: Path, verbose: bool) -> Path:
     obj = BUILD / (src.stem + ".o")
     cmd = [nvcc(), *ARCH, *NVCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(src), "-o", str(obj)]
@@ -63,8 +95,9 @@ def _compile(src: Path, verbose: bool) -> Path:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile (when sources changed) and return the path of libexl3b200.so."""
+    """Compile (when sources changed) and return the path of libexl3b200.so; the torch binding too."""
     if not force and up_to_date():
+        build_binding()
         return LIB
     BUILD.mkdir(exist_ok=True)
     srcs = sources()
@@ -76,6 +109,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    build_binding(force)
     return LIB
 
 
