@@ -11,6 +11,10 @@
 //            column) through distributed shared memory.
 // A draw by inverting the cumulative distribution would need a prefix sum over the vocabulary and give another token for
 // another order of summation; the race depends on each w alone.
+//
+// 64 sequences of up to 8 rows with as many draft rows but one, 151,936 columns of bf16, 190 MB: 52 us (3.6 TB/s, 0.56 of a
+// measured copy): about 31 for the statistics, near a copy's rate, the rest for a race that cannot begin before all of a
+// sequence's statistics are known. One sequence of 4 rows: 12.5 us, two launches and two rounds of loads.
 #include <cuda_runtime.h>
 
 #include <type_traits>
@@ -26,7 +30,7 @@ namespace exl3 {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kStatThreads = 128, kStatWarps = kStatThreads / 32;
-constexpr int kStatPer = 32;                          // columns a thread keeps in registers
+constexpr int kStatVecs = 8;                          // 16-byte vectors a thread keeps in registers
 constexpr int kDecideWarps = 16;                      // most of a CTA
 constexpr int kVerifyCluster = 8;
 
@@ -53,12 +57,39 @@ __device__ __forceinline__ void take_first(float& v, int& i, float ov, int oi)
 }
 
 // ------------------------------------------------------------------------------ statistics
-// Small CTAs, so that some load while others reduce. The row's columns from its first 16-byte boundary on go to the chunks as whole vectors; the few
-// before it are chunk 0's, the last vector may be partial.
+template <typename T> __device__ __forceinline__ uint32_t lowest_word();       // -inf in each place of a word
+template <> __device__ __forceinline__ uint32_t lowest_word<__half>() { return 0xFC00FC00u; }
+template <> __device__ __forceinline__ uint32_t lowest_word<__nv_bfloat16>() { return 0xFF80FF80u; }
+template <> __device__ __forceinline__ uint32_t lowest_word<float>() { return 0xFF800000u; }
+
+// Value i of a word of the row (two of a 16-bit type).
 template <typename T>
-__global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const VerifyArgs a)
+__device__ __forceinline__ float word_value(uint32_t w, int i)
 {
-    constexpr int PER = kStatPer, VEC = 16 / sizeof(T), N = PER / VEC;
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i ? w & 0xFFFF0000u : w << 16);
+    else return __half2float(__ushort_as_half((unsigned short)(i ? w >> 16 : w)));
+}
+
+// Larger values of two words place by place; of a number and a NaN, the number.
+template <typename T>
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    if constexpr (sizeof(T) == 4) r = __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// Small CTAs, so that some load while others reduce; a thread keeps its columns as they are stored, which leaves registers for
+// 8 CTAs an SM with 128 bytes a thread in flight (6 without the few spilled bytes: 54.0 us against 52.6 for the 190 MB above;
+// columns unpacked to fp32, 5 CTAs: 58.7). The row's columns from its first 16-byte boundary on go to the chunks as
+// whole vectors; the few before it are chunk 0's, the last vector may be partial.
+template <typename T>
+__global__ void __launch_bounds__(kStatThreads, 8) verify_stats_kernel(const VerifyArgs a)
+{
+    constexpr int VEC = 16 / sizeof(T), PW = 4 / sizeof(T), N = kStatVecs;     // columns of a vector, of a word; vectors
     __shared__ float sv[kStatWarps];
     __shared__ int si[kStatWarps];
     pdl_trigger();
@@ -69,13 +100,14 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
     const T* x = is_draft ? static_cast<const T*>(a.draft) + (r - a.rows) * a.draft_ld
                           : static_cast<const T*>(a.target) + r * a.target_ld;
     const int head = min(a.n, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-    const int first = head + chunk * (kStatThreads * PER) + tid * VEC;
+    const int first = head + chunk * (kStatThreads * N * VEC) + tid * VEC;
+    const uint32_t none = lowest_word<T>();
     uint4 w[N];
-    auto fetch = [&]() {                              // whole vectors; the row's last may be partial
+    auto fetch = [&]() {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int at = first + k * kStatThreads * VEC;
-            w[k] = at + VEC <= a.n ? *reinterpret_cast<const uint4*>(x + at) : make_uint4(0, 0, 0, 0);
+            w[k] = at + VEC <= a.n ? *reinterpret_cast<const uint4*>(x + at) : make_uint4(none, none, none, none);
         }
     };
     // a target row's logits are on their way while its temperature is looked up
@@ -88,26 +120,28 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
         if (greedy) return;                           // q is one-hot: the row is not looked at
         fetch();
     }
-    float v[PER + 1];
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-        const T* e = reinterpret_cast<const T*>(&w[k]);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[k * VEC + i] = to_f32(e[i]);
-    }
-    if (head + (chunk + 1) * (kStatThreads * PER) > a.n) {             // the row ends in this chunk
+    if (head + (chunk + 1) * (kStatThreads * N * VEC) > a.n) {         // the row ends in this chunk: its last vector
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int at = first + k * kStatThreads * VEC;
+            if (at < a.n && at + VEC > a.n) {
+                uint32_t q[4] = {none, none, none, none};
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                if (at + VEC > a.n) v[k * VEC + i] = at + i < a.n ? to_f32(x[at + i]) : -INFINITY;
+                for (int i = 0; i < VEC; ++i)
+                    if (at + i < a.n) {
+                        if constexpr (PW == 1) q[i] = reinterpret_cast<const uint32_t*>(x)[at + i];
+                        else q[i / 2] = __byte_perm(q[i / 2], reinterpret_cast<const unsigned short*>(x)[at + i], i & 1 ? 0x5410 : 0x3254);
+                    }
+                w[k] = make_uint4(q[0], q[1], q[2], q[3]);
+            }
         }
     }
-    v[PER] = chunk == 0 && tid < head ? to_f32(x[tid]) : -INFINITY;
-    float m = v[PER];
+    const float xh = chunk == 0 && tid < head ? to_f32(x[tid]) : -INFINITY;
+    uint32_t most = none;
 #pragma unroll
-    for (int i = 0; i < PER; i += 2) m = max3(m, v[i], v[i + 1]);
+    for (int k = 0; k < N; ++k) most = word_max<T>(most, word_max<T>(word_max<T>(w[k].x, w[k].y), word_max<T>(w[k].z, w[k].w)));
+    float m = fmaxf(xh, word_value<T>(most, 0));
+    if (PW == 2) m = fmaxf(m, word_value<T>(most, 1));
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) sv[warp] = m;
@@ -116,14 +150,21 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
 #pragma unroll
     for (int o = kStatWarps / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float base = m == -INFINITY ? 0.f : m, c = (greedy ? 1.f : 1.f / temp) * kLog2e;
-    // the maximum is taken off before scaling: the lowest value of the type scaled by 1 / T would overflow
+    // the maximum is taken off before scaling: the type's lowest value times 1 / T would overflow
     const uint64_t c2 = f2(c, c), zero = f2(0.f, 0.f), off = f2(-base, -base);
-    uint64_t s2 = f2(ex2((v[PER] - base) * c), 0.f);
-#pragma unroll
-    for (int i = 0; i < PER; i += 2) {
+    uint64_t s2 = f2(ex2((xh - base) * c), 0.f);
+    auto add2 = [&](float u, float v) {
         float e0, e1;
-        f2_get(f2_fma(f2_add(f2(v[i], v[i + 1]), off), c2, zero), e0, e1);
+        f2_get(f2_fma(f2_add(f2(u, v), off), c2, zero), e0, e1);
         s2 = f2_add(s2, f2(ex2(e0), ex2(e1)));
+    };
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const uint32_t q[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+        for (int i = 0; i < 4; i += 3 - PW)
+            if (PW == 2) add2(word_value<T>(q[i], 0), word_value<T>(q[i], 1));
+            else add2(word_value<T>(q[i], 0), word_value<T>(q[(i + 1) & 3], 0));
     }
     float s0, s1;
     f2_get(s2, s0, s1);
@@ -131,11 +172,14 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
     int at = 0x7fffffff;
     if (greedy) {
 #pragma unroll
-        for (int i = PER - 1; i >= 0; --i)
-            if (v[i] == m) at = first + (i / VEC) * kStatThreads * VEC + i % VEC;
-        if (chunk == 0 && tid < head && v[PER] == m) at = tid;
+        for (int k = N - 1; k >= 0; --k) {
+            const uint32_t q[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
 #pragma unroll
-        for (int o = 16; o; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
+            for (int i = VEC - 1; i >= 0; --i)
+                if (word_value<T>(q[i / PW], i % PW) == m) at = first + k * kStatThreads * VEC + i;
+        }
+        if (chunk == 0 && tid < head && xh == m) at = tid;
+        at = __reduce_min_sync(0xffffffffu, at);
     }
     __syncthreads();
     if (lane == 0) {
@@ -146,9 +190,9 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
     if (tid == 0) {
         float sum = 0.f;
         int col = 0x7fffffff;
-        for (int w = 0; w < kStatWarps; ++w) {
-            sum += sv[w];
-            col = min(col, si[w]);
+        for (int k = 0; k < kStatWarps; ++k) {
+            sum += sv[k];
+            col = min(col, si[k]);
         }
         a.stats[blockIdx.x] = make_float4(m, sum, __int_as_float(col), 0.f);
     }
@@ -391,9 +435,14 @@ __global__ void __launch_bounds__(32 * kDecideWarps) verify_decide_kernel(const 
     }
 }
 
-static int verify_chunks(int n) { return (n + kStatPer * kStatThreads - 1) / (kStatPer * kStatThreads); }
+static int verify_chunks(int n, int esz)
+{
+    const int columns = kStatVecs * kStatThreads * (16 / esz);
+    return (n + columns - 1) / columns;
+}
 
-static size_t verify_bytes(int rows, int seqs, int n) { return (size_t)(2ll * rows - seqs) * verify_chunks(n) * sizeof(float4); }
+// Sized for the widest type, so that the query needs no dtype.
+static size_t verify_bytes(int rows, int seqs, int n) { return (size_t)(2ll * rows - seqs) * verify_chunks(n, 4) * sizeof(float4); }
 
 template <typename T>
 static int launch_verify(const VerifyArgs& a, cudaStream_t s)
@@ -448,7 +497,7 @@ extern "C" int exl3_verify_drafts(const void* target, long long target_ld, const
     a.out = tokens_out; a.count = count; a.prob = accept_prob;
     a.stats = static_cast<float4*>(workspace);
     a.rows = rows; a.seqs = seqs; a.n = n; a.max_drafts = max_drafts;
-    a.chunks = verify_chunks(n);
+    a.chunks = verify_chunks(n, esz);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (dtype) {
     case EXL3_F16: return launch_verify<__half>(a, s);
