@@ -3,9 +3,8 @@
 //
 //   xn = x * rsqrt(mean(x^2) + eps) * w ;  (a, b) = (xn[c], xn[c + R]) -> (a cos - b sin, b cos + a sin), c < R
 //
-// A lane holds four columns of each half of a head, so that the norm's sum is a few shuffles and the rotation needs none. Bound by the
-// rows' bytes where there are many (3428 rows of 40 + 2 x 8 heads of 128, 100 MB: 24 us, 4.1 TB/s, 0.63 of a measured copy, in a pass too short to
-// reach a copy's rate), by launch and two dependent loads (row's sequence, its page) where there are few (3.1 us).
+// Bound by the rows' bytes where there are many (3428 rows of 40 + 2 x 8 heads of 128, 100 MB in 23.7 us, 4.2 TB/s, 0.65 of a
+// measured copy, which so short a pass does not reach), by launch and dependent loads where there are few (2.9 us).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -59,10 +58,11 @@ __device__ __forceinline__ void store4(C* p, const float* x)
 // A warp handles one row and every per_row-th group of its heads (PER heads at once). A lane holds two runs of four elements of
 // a head, the two sides of its rotation pairs (c and c + rope_half), so rotating needs no exchange; lanes past the rotated
 // part hold two runs of what passes unchanged. What belongs to the row (its sequence, page, rotation) is looked up once.
-// Bound by the bytes for a long batch, whose loads are U groups deep per warp, and by latency for single tokens,
-// whose head groups each get a warp.
+// The loads are U groups deep, the first of them under way while the row is looked up (a single token 3.15 -> 2.86 us); asking for
+// the next round's within a round was slower (50.6 us for the 3428 rows), and so were two or three groups at more CTAs (25.2
+// to 29.5). Six CTAs an SM, since a warp that handles a whole row runs long: five took a second wave (31.9 us).
 template <typename T, typename C, int HD, bool VEC>
-__global__ void __launch_bounds__(128) paged_post_kernel(const PagedPostArgs a)
+__global__ void __launch_bounds__(128, 6) paged_post_kernel(const PagedPostArgs a)
 {
     constexpr int L = HD / 8;                            // lanes of one head
     constexpr int PER = 32 / L;                          // heads a warp handles at once
@@ -78,6 +78,20 @@ __global__ void __launch_bounds__(128) paged_post_kernel(const PagedPostArgs a)
     const int c0 = rotated ? 4 * sub : R + 4 * sub;      // past the rotated part: 2 R + 4 (sub - R / 4)
     const int c1 = rotated ? c0 + R : c0 + HD / 2 - R;
     pdl_wait();
+    // the heads' loads do not depend on what is looked up for the row
+    const int heads = a.hq + 2 * b.hkv, stride = a.per_row * PER;
+    const T* const q = static_cast<const T*>(a.q) + row * a.sq;
+    const T* const k = static_cast<const T*>(a.k) + row * a.sk - (size_t)a.hq * HD;
+    const T* const v = static_cast<const T*>(a.v) + row * a.sv - (size_t)(a.hq + b.hkv) * HD;
+    uint2 in[U][2];
+    auto fetch = [&](int u, int g) {
+        const int h = min(g + lane / L, heads - 1);
+        const T* src = (h < a.hq ? q : h < a.hq + b.hkv ? k : v) + (size_t)h * HD;
+        in[u][0] = load4<T, VEC>(src + c0);
+        in[u][1] = load4<T, VEC>(src + c1);
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) fetch(u, part * PER + u * stride);
     const int s = seq_of_row(b.cu_rows, b.seqs, row, lane);
     const int pos = b.lens[s] - b.cu_rows[s + 1] + row;
     const bool pad = pos < 0, known = pos < a.rope_rows;
@@ -91,28 +105,19 @@ __global__ void __launch_bounds__(128) paged_post_kernel(const PagedPostArgs a)
     }
     uint2 wq0{}, wq1{}, wk0{}, wk1{};
     if (a.qw) {
-        wq0 = load4<T, false>(static_cast<const T*>(a.qw) + c0);
-        wq1 = load4<T, false>(static_cast<const T*>(a.qw) + c1);
+        wq0 = load4<T, VEC>(static_cast<const T*>(a.qw) + c0);
+        wq1 = load4<T, VEC>(static_cast<const T*>(a.qw) + c1);
     }
     if (a.kw) {
-        wk0 = load4<T, false>(static_cast<const T*>(a.kw) + c0);
-        wk1 = load4<T, false>(static_cast<const T*>(a.kw) + c1);
+        wk0 = load4<T, VEC>(static_cast<const T*>(a.kw) + c0);
+        wk1 = load4<T, VEC>(static_cast<const T*>(a.kw) + c1);
     }
-    const int heads = a.hq + 2 * b.hkv, stride = a.per_row * PER;
-    const T* const q = static_cast<const T*>(a.q) + row * a.sq;
-    const T* const k = static_cast<const T*>(a.k) + row * a.sk - (size_t)a.hq * HD;
-    const T* const v = static_cast<const T*>(a.v) + row * a.sv - (size_t)(a.hq + b.hkv) * HD;
     C* const qo = static_cast<C*>(a.q_out) + (size_t)row * a.hq * HD;
     const size_t slot = ((size_t)max(page, 0) * b.hkv * b.page_size + (pos & (b.page_size - 1))) * HD;
     for (int g0 = part * PER; g0 < heads; g0 += U * stride) {
-        uint2 in[U][2];
+        if (g0 != part * PER)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int h = min(g0 + u * stride + lane / L, heads - 1);
-            const T* src = (h < a.hq ? q : h < a.hq + b.hkv ? k : v) + (size_t)h * HD;
-            in[u][0] = load4<T, VEC>(src + c0);
-            in[u][1] = load4<T, VEC>(src + c1);
-        }
+            for (int u = 0; u < U; ++u) fetch(u, g0 + u * stride);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int h = g0 + u * stride + lane / L;
@@ -214,9 +219,10 @@ extern "C" int exl3_paged_qkv_post(const exl3_paged_desc* batch, const void* q, 
     a.cos_t = cos_table; a.sin_t = sin_table;
     a.q_out = q_out; a.status = status; a.eps = eps;
     a.hq = hq; a.rope_rows = rope_rows; a.rope_half = rope_half;
-    const bool vec = aligned(q, 8) && aligned(k, 8) && aligned(v, 8) && q_stride % 4 == 0 && k_stride % 4 == 0 && v_stride % 4 == 0;
+    const bool vec = aligned(q, 8) && aligned(k, 8) && aligned(v, 8) && aligned(q_norm_w, 8) && aligned(k_norm_w, 8) &&
+                     q_stride % 4 == 0 && k_stride % 4 == 0 && v_stride % 4 == 0;
     // A row's warps: one for every four groups (one round of loads) while that fits the SMs' warp slots, then fewer and longer
-    // ones. Measured at 56 heads of 128, us with 1 / 2 / 7 / 28 warps a row: 1 row 10.5 / 6.8 / 3.2 / 3.1, 600 rows 12.4 /
+    // ones. Measured at 56 heads of 128, us with 1 / 2 / 7 / 28 warps a row: 1 row 10.5 / 6.8 / 2.9 / 3.1, 600 rows 12.4 /
     // 11.2 / 6.8 / 15.2, 3428 rows 24.1 / 25.7 / 28.2 / 83.9.
     const int per = 32 / (batch->head_dim / 8), groups = (hq + 2 * batch->hkv + per - 1) / per;
     const int warps = 32 * device_sm_count();
