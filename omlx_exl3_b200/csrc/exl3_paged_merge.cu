@@ -129,6 +129,12 @@ __global__ void __launch_bounds__(kPmThreads) paged_merge_kernel(const __grid_co
     const bool is_few = blockIdx.z == 1 || !tiles.items;
     const PaArgs& a = is_few ? few : tiles;
     const PaItem g = a.items[blockIdx.x];
+    if (blockIdx.z == 0) {                            // rows behind the last sequence's are padding: zeros
+        const size_t row16 = (size_t)a.hq * HD / 8, n = row16 * a.b.rows, threads = (size_t)gridDim.x * gridDim.y * kPmThreads;
+        const size_t first = row16 * max(a.b.cu_rows[a.b.seqs], 0);
+        for (size_t i = first + (blockIdx.y * gridDim.x + blockIdx.x) * kPmThreads + threadIdx.x; i < n; i += threads)
+            reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
+    }
     if (g.parts < 2) return;
     if (is_few) merge_item<C, HD, kPaFew, 1>(a, g);
     else merge_item<C, HD, kPaRows, 2>(a, g);

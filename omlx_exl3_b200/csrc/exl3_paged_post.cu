@@ -93,8 +93,8 @@ __global__ void __launch_bounds__(128, 6) paged_post_kernel(const PagedPostArgs 
 #pragma unroll
     for (int u = 0; u < U; ++u) fetch(u, part * PER + u * stride);
     const int s = seq_of_row(b.cu_rows, b.seqs, row, lane);
-    const int pos = b.lens[s] - b.cu_rows[s + 1] + row;
-    const bool pad = pos < 0, known = pos < a.rope_rows;
+    const int end = b.cu_rows[s + 1], pos = b.lens[s] - end + row;
+    const bool pad = pos < 0 || row >= end || row < b.cu_rows[0], known = pos < a.rope_rows;
     const int page = page_of(b, s, pos);
     if (!pad && (!known || page < 0) && lane == 0 && part == 0) atomicOr(a.status, kStatusPagedRange);
     const bool append = !pad && known && page >= 0, has_q = !pad && known;

@@ -28,7 +28,11 @@
 
 namespace exl3 {
 
-constexpr float kLog2e = 1.4426950408889634f;
+// log2(e) / T; T far outside the range of logits counts as one at its end, so that the factor is neither 0 nor infinite.
+__device__ __forceinline__ float exponent_scale(float temperature, bool greedy)
+{
+    return 1.4426950408889634f / (greedy ? 1.f : fminf(fmaxf(temperature, 1e-30f), 1e30f));
+}
 constexpr int kStatThreads = 128, kStatWarps = kStatThreads / 32;
 constexpr int kStatVecs = 8;                          // 16-byte vectors a thread keeps in registers
 constexpr int kDecideWarps = 16;                      // most of a CTA
@@ -149,7 +153,7 @@ __global__ void __launch_bounds__(kStatThreads, 8) verify_stats_kernel(const Ver
     m = sv[lane & (kStatWarps - 1)];
 #pragma unroll
     for (int o = kStatWarps / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base = m == -INFINITY ? 0.f : m, c = (greedy ? 1.f : 1.f / temp) * kLog2e;
+    const float base = m == -INFINITY ? 0.f : m, c = exponent_scale(temp, greedy);
     // the maximum is taken off before scaling: the type's lowest value times 1 / T would overflow
     const uint64_t c2 = f2(c, c), zero = f2(0.f, 0.f), off = f2(-base, -base);
     uint64_t s2 = f2(ex2((xh - base) * c), 0.f);
@@ -279,7 +283,7 @@ __global__ void __launch_bounds__(32 * kDecideWarps) verify_decide_kernel(const 
     const bool sane = lo >= s && hi > lo && hi <= a.rows && hi - s - 1 <= a.rows - a.seqs;
     const float temp = a.temperature ? a.temperature[s] : 1.f;
     const bool greedy = !(temp > 0.f);
-    const float c = (greedy ? 1.f : 1.f / temp) * kLog2e;
+    const float c = exponent_scale(temp, greedy);
     const int judged = sane ? hi - lo - 1 : 0;        // drafts of this sequence
     const int limit = min(judged, a.max_drafts);
 

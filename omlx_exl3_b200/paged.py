@@ -11,8 +11,8 @@ is the part of a server that sits between the EXL3 projections:
 A batch is cu_rows (seqs + 1), lens (seqs) and page_table (seqs, cols), all int32 on the device: sequence s feeds
 rows cu_rows[s] .. cu_rows[s + 1] - 1 and holds lens[s] positions once they are appended, so its row i is at
 position lens[s] - rows[s] + i; position p lives in page page_table[s, p // page_size]. Rows at negative positions
-are padding: nothing is appended and the output is zero (a captured graph's unused slots have lens 0). The
-kernels read the tables themselves, so no call waits for the host and a captured graph follows their contents.
+and rows from cu_rows[seqs] on are padding: nothing is appended and the output is zero (a captured graph's unused
+slots have no rows, or lens 0). The kernels read the tables themselves, so no call waits for the host and a captured graph follows their contents.
 
 Calls run on the current stream. Tables that name something outside the pool set a bit in a per-device status
 word, as a pipeline wait that gave up does: check_paged_status() raises on it.

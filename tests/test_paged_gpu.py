@@ -79,6 +79,30 @@ def test_attn_padding_rows_and_empty_sequences(cuda, hd):
     assert _attn(q[:0], none).shape == (0, 6, hd)
 
 
+@pytest.mark.parametrize("rows,lens", [([1, 2], [40, 130]), ([200, 1, 0], [300, 77, 0]), ([0], [16])])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_rows_behind_the_last_sequence_are_padding(cuda, rows, lens, hd):
+    """A call of more rows than the sequences have (a captured graph's width): zeros for them, nothing appended, and the
+    others as in a call without them."""
+    from omlx_exl3_b200 import check_paged_status, paged_qkv_post
+    n, more, hq, hkv = sum(rows), 5, 4, 2
+    b = make_batch(rows, lens, hkv, hd, 16, torch.float16, cuda, seed=40, spare=1)
+    q = torch.randn((n + more, hq, hd), generator=torch.Generator().manual_seed(41)).half().to(cuda)
+    out = torch.full_like(q, 7.0)
+    assert _attn(q, b, out=out) is out
+    assert torch.equal(out[:n], _attn(q[:n], b)) and not out[n:].any()
+    y = torch.randn((n + more, (hq + 2 * hkv) * hd), device=cuda).half()
+    cos, sin = (t.to(cuda) for t in _rope_tables(512, hd // 2))
+    split = [hq * hd, hkv * hd, hkv * hd]
+    pages = [(b["kp"].clone(), b["vp"].clone()) for _ in range(2)]
+    outs = [paged_qkv_post(*x.split(split, 1), None, None, 1e-6, cos, sin, *p, b["table"], b["cu"], b["lens"])
+            for x, p in zip((y, y[:n]), pages)]
+    assert torch.equal(outs[0][:n], outs[1]) and not outs[0][n:].any()
+    for x, z in zip(*pages):
+        assert torch.equal(x.view(torch.int16), z.view(torch.int16))
+    check_paged_status(cuda)
+
+
 def test_attn_sharp_and_growing_scores(cuda):
     """Scores of +-60 whose maximum moves along the cache: the running maximum has to follow it."""
     dtype = torch.float16

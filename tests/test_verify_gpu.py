@@ -115,6 +115,15 @@ def test_verify_masked_logits(cuda, dtype):
     assert got[0][2].tolist() == [-1] * 4 and int(got[1][2]) == 1 and int(got[0][5, 0]) == -1
 
 
+@pytest.mark.parametrize("dist", [True, False])
+def test_verify_extreme_temperatures(cuda, dist):
+    """Temperatures whose reciprocal is no fp32 number, or nearly none: as good as greedy, as good as uniform."""
+    target, tokens, cu, u, noise, draft, _ = _inputs([3, 3, 3, 3], 900, torch.float32, seed=12)
+    target[1, 5:80] = draft[1, 9:100] = float("-inf")
+    temp = torch.tensor([1e-39, 1e-32, 1e35, 3e38])
+    _check(cuda, target, tokens, cu, u, noise, 2, draft if dist else None, temp)
+
+
 def test_verify_greedy_ties_and_foreign_drafts(cuda):
     """Equal logits: the first is the greedy token. Drafted ids outside the vocabulary are never accepted."""
     n = 5000
