@@ -216,8 +216,10 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;                 // S of slot i at column 128 i, O at 256 + HD i
-    pdl_trigger();
+    // What this kernel reads is complete once it may go on; the kernel for few rows reads the same and begins behind this
+    // trigger on SMs that have no tiles (left).
     pdl_wait();
+    pdl_trigger();
 
     PaSched sched(a);
     PaSeg g{};
@@ -772,9 +774,10 @@ extern "C" int exl3_paged_attn(const exl3_paged_desc* batch, const void* q, long
     tiles.parts = base + w.tile_parts;
     tiles.lo = tiles_only ? 0 : hi;
     tiles.hi = 0x7fffffff;
-    if (!tiles_only)
-        if (int e = pa_launch_few(few, s)) return e;
+    few.behind = !few_only;
     if (!few_only)
         if (int e = pa_launch_tiles(tiles, s)) return e;
+    if (!tiles_only)
+        if (int e = pa_launch_few(few, s)) return e;
     return pa_launch_merge(few_only ? nullptr : &tiles, tiles_only ? nullptr : &few, attn_ctas(), s);
 }

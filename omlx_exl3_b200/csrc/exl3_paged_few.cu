@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
     const uint32_t ring = smem_addr(pf_sm) + warp * S::kDepth * S::kSlot;
     float* merge = reinterpret_cast<float*>(pf_sm + kPfWarps * S::kDepth * S::kSlot);
     pdl_trigger();
-    pdl_wait();
+    if (!a.behind) pdl_wait();
 
     PaSched sched(a);
     sched.start(blockIdx.x, gridDim.x, lane);
@@ -327,6 +327,7 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
     }
     if (threadIdx.x == 0) pa_record(a, any, g, any ? min(8 * NQ, g.rows * a.grp - g.p0) : 0, 8 * NQ);   // g: the last segment
     cp_async_wait<0>();
+    if (a.behind) pdl_wait();                         // so that the merge, which waits for this kernel, finds the tiles' parts too
 }
 
 template <typename C, int HD, int NQ>

@@ -34,6 +34,7 @@ struct PaArgs {
     float scale_log2;
     int hq, grp, span, item;
     uint32_t grp_magic;                               // ceil(2^32 / grp): x / grp = umulhi(x, grp_magic) for x < 2^25 (0: grp is 1)
+    int behind;                                       // launched behind the tile kernel, which it need not wait for to begin
     int lo, hi;                                       // sequences of lo < rows * grp <= hi are this kernel's
 };
 
