@@ -757,7 +757,9 @@ extern "C" int exl3_paged_attn(const exl3_paged_desc* batch, const void* q, long
     // start; 16 rows at a time read the keys and values once per 16. Measured, us with sequences of up to 32 / up to 64
     // packed rows on the latter: 9 of 1 to 8 rows (4200 positions, group 5) 28.3 / 18.2; 16 of 8 rows over 2000 (40 each)
     // 49.2 / 67.5; 64 of 4 rows (20 each) 38.8, and 51.0 on tiles. A batch with a row per sequence at most is taken for
-    // single tokens: one launch, right whatever the rows are.
+    // single tokens: one launch, right whatever the rows are. Where both
+    // run, the kernel for few rows comes second and waits for the tiles at its end only: 13 sequences of 1 to 777 rows 54.6 us,
+    // and 58.7 one after the other.
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const long long packed = (long long)batch->rows * a.grp;
     const int hi = packed <= 32ll * batch->seqs ? 64 : 32;
