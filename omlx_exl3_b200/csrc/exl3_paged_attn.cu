@@ -753,16 +753,17 @@ extern "C" int exl3_paged_attn(const exl3_paged_desc* batch, const void* q, long
     a.grp_magic = a.grp == 1 ? 0u : (uint32_t)(((1ull << 32) + a.grp - 1) / a.grp);
     if (!pa_list_fits(a, 8)) return EXL3_E_SHAPE;
     // Which kernel takes a sequence goes by its packed rows, which only the device knows: the host launches what they may need,
-    // from their average and what it knows of the most. A 128-row tile costs the same however empty it is, but more at the
-    // start; 16 rows at a time read the keys and values once per 16. Measured, us with sequences of up to 32 / up to 64
-    // packed rows on the latter: 9 of 1 to 8 rows (4200 positions, group 5) 28.3 / 18.2; 16 of 8 rows over 2000 (40 each)
-    // 49.2 / 67.5; 64 of 4 rows (20 each) 38.8, and 51.0 on tiles. A batch with a row per sequence at most is taken for
-    // single tokens: one launch, right whatever the rows are. Where both
-    // run, the kernel for few rows comes second and waits for the tiles at its end only: 13 sequences of 1 to 777 rows 54.6 us,
-    // and 58.7 one after the other.
+    // from their average and what it knows of the most. A 128-row tile costs the same however empty it is, and more at the
+    // start, which counts while the SMs outnumber the pairs of a sequence and a kv head; 16 rows at a time read the keys and
+    // values once per 16. Measured, us with sequences of up to 32 / up to 64 packed rows on the latter, each of 1 to 8 rows in
+    // groups of 5 heads: 9 over 1000 positions of 8 kv heads 22.0 / 18.9, 16 26.8 / 21.9, 16 over 8000 41.4 / 44.3, 32 57.4 / 65.5, 64
+    // 98.2 / 122.3, 128 127.4 / 142.4; of 4 kv heads 9 over 8000 26.8 / 23.0, 32 39.6 / 38.9, 64 61.6 / 71.6. (Up to 16: 64 over
+    // 8000 95.5, but 1 to 5 rows 42.7 / 39.4 at 16 / 32.) A batch with a row per sequence at most is taken for single tokens:
+    // one launch, right whatever the rows are. Where both run, the kernel for few rows comes second and waits for the tiles at
+    // its end only: 13 sequences of 1 to 777 rows 54.6 us, and 58.7 one after the other.
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const long long packed = (long long)batch->rows * a.grp;
-    const int hi = packed <= 32ll * batch->seqs ? 64 : 32;
+        const int hi = packed <= 32ll * batch->seqs && (long long)batch->seqs * batch->hkv <= attn_ctas() ? 64 : 32;
     const long long most = max_rows > 0 && max_rows < batch->rows ? (long long)max_rows * a.grp : packed;
     const bool few_only = most <= hi || (batch->rows <= batch->seqs && a.grp <= hi);
     const bool tiles_only = !few_only && (batch->seqs == 1 || a.grp > hi);
