@@ -369,3 +369,52 @@ def test_append_then_attend_matches_one_long_prompt(cuda):
     whole, parts = feed([n]), feed([1, 1, 16, 100, 3, 128, 1, 83])
     err = (whole.float() - parts.float()).abs().max()
     assert err <= 4 * UNIT[torch.float16] * 4.5                       # |v| < 4.5: p rounded twice, the output twice
+
+
+@pytest.mark.parametrize("hd,hq,hkv", [(128, 10, 2), (64, 4, 4)])
+def test_steps_of_mixed_batches_in_a_graph(cuda, hd, hq, hkv):
+    """Appends and attention of chunks and single tokens, step after step in one graph without a gap: each step's attention
+    reads what the step before it just wrote, as when every call is waited for."""
+    from omlx_exl3_b200 import check_paged_status, paged_attn, paged_qkv_post
+    steps, rows = 4, [260, 1, 4, 0, 1, 33]
+    lens = [[260 * (i + 1), 900 + i, 130 + 4 * i, 7, 1 + i, 2000 + 33 * i] for i in range(steps)]
+    b = make_batch(rows, lens[-1], hkv, hd, 32, torch.float16, cuda, seed=50, fill=0.0)
+    n = sum(rows)
+    gen = torch.Generator().manual_seed(51)
+    y = [torch.randn((n, (hq + 2 * hkv) * hd), generator=gen).half().to(cuda) for _ in range(steps)]
+    at = [torch.tensor(x, dtype=torch.int32, device=cuda) for x in lens]
+    w = (1 + 0.1 * torch.randn(hd, generator=gen)).half().to(cuda)
+    cos, sin = (x.to(cuda) for x in _rope_tables(2200, hd // 2))
+    first = b["kp"].clone(), b["vp"].clone()
+
+    def run(wait):
+        outs = []
+        for i in range(steps):
+            q = paged_qkv_post(*y[i].split([hq * hd, hkv * hd, hkv * hd], 1), w, w, 1e-6, cos, sin, b["kp"], b["vp"], b["table"],
+                               b["cu"], at[i])
+            if wait:
+                torch.cuda.synchronize()
+            outs.append(paged_attn(q, b["kp"], b["vp"], b["table"], b["cu"], at[i]))
+            if wait:
+                torch.cuda.synchronize()
+        return outs
+
+    def restore():
+        b["kp"].copy_(first[0])
+        b["vp"].copy_(first[1])
+
+    want = run(True)
+    pages = b["kp"].clone(), b["vp"].clone()
+    g = torch.cuda.CUDAGraph()
+    restore()
+    with torch.cuda.graph(g):
+        outs = run(False)
+    for _ in range(5):
+        restore()
+        for o in outs:
+            o.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, z) for x, z in zip(outs, want))
+        assert torch.equal(b["kp"], pages[0]) and torch.equal(b["vp"], pages[1])
+    check_paged_status(cuda)
