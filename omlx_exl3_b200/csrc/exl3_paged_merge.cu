@@ -1,7 +1,7 @@
 // Merges the partial results of paged-attention items that were cut between CTAs, in CTA order:
 //   m = max m_k, out = sum_k exp2((m_k - m) c) O_k / sum_k exp2((m_k - m) c) l_k.
 //
-// grid (CTAs of the attention kernels, blocks of an item, lists): block x looks at the item that started in CTA x's share.
+// grid (CTAs of the attention kernels, blocks of an item of few rows, then of one of tiles): block x looks at the item that started in CTA x's share.
 // (One CTA, the last to finish its part, merging alone was measured first: 40 rows of 33 parts are 0.7 MB, 25 us for one
 // SM.) The time is L2 latency, so a quad's parts are loaded four at a time, and by four threads where there are many.
 #include <cuda_runtime.h>
@@ -15,8 +15,9 @@
 namespace exl3 {
 
 constexpr int kPmThreads = 128;
-constexpr int kPmBlocks = 16;                         // of an item of tiles
-constexpr int kPmFewBlocks = 4;                       // of one of few rows
+constexpr int kPmBlocks = 16;                         // of an item of tiles (8, 12 and 32 were slower: 68.3, 64.9 and 63.1 us against
+                                                      // 62.7 for 512 rows over 4096 positions of 40 / 8 heads)
+constexpr int kPmFewBlocks = 8;                       // of one of few rows (4: 10.7 us against 9.2 for one row over 4097)
 
 // A column quad of an item: its tile, its row there, its place in the tile's parts.
 struct PmQuad {
@@ -60,14 +61,14 @@ struct PmSum {
 
 // G neighbouring threads share a quad's parts (thread k takes parts k, k + G, ...), K parts' loads in flight each.
 template <typename C, int HD, int ROWS, int TILES, int G>
-__device__ __forceinline__ void merge_item(const PaArgs& a, const PaItem& g)
+__device__ __forceinline__ void merge_item(const PaArgs& a, const PaItem& g, int block, int blocks)
 {
     constexpr int K = 4, QW = 32 / G;                 // quads of a warp
     constexpr size_t kMl = PaPart<HD, ROWS>::kMl;
     const float c = a.scale_log2;
     const int lane = threadIdx.x & 31, part0 = lane / QW;
-    const int n = g.used * (HD / 4), stride = kPmThreads / G * gridDim.y;
-    for (int e0 = (blockIdx.y * (kPmThreads / 32) + (threadIdx.x >> 5)) * QW; e0 < n; e0 += stride) {
+    const int n = g.used * (HD / 4), stride = kPmThreads / G * blocks;
+    for (int e0 = (block * (kPmThreads / 32) + (threadIdx.x >> 5)) * QW; e0 < n; e0 += stride) {
         const int e = e0 + lane % QW;
         const PmQuad q = pm_quad<HD, TILES>(g, min(e, n - 1));
         PmSum p;
@@ -76,18 +77,22 @@ __device__ __forceinline__ void merge_item(const PaArgs& a, const PaItem& g)
             float4 y[K];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const uint8_t* pt = pa_part<HD, ROWS, TILES>(a.parts, g.c0, g.c0 + min(k0 + k * G, g.parts - 1), q.tile);
-                w[k] = __ldcg(reinterpret_cast<const float2*>(pt + kMl) + q.row);
-                y[k] = __ldcg(reinterpret_cast<const float4*>(pt) + q.at);
+                w[k] = make_float2(-INFINITY, 0.f);
+                y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k0 + k * G < g.parts) {
+                    const uint8_t* pt = pa_part<HD, ROWS, TILES>(a.parts, g.c0, g.c0 + k0 + k * G, q.tile);
+                    w[k] = __ldcg(reinterpret_cast<const float2*>(pt + kMl) + q.row);
+                    y[k] = __ldcg(reinterpret_cast<const float4*>(pt) + q.at);
+                }
             }
             float now = p.top;
 #pragma unroll
-            for (int k = 0; k < K; ++k) now = fmaxf(now, w[k].x);      // past the last part: the last one's again
+            for (int k = 0; k < K; ++k) now = fmaxf(now, w[k].x);
             p.scale(pa_weight(p.top, now, c));
             p.top = now;
 #pragma unroll
             for (int k = 0; k < K; ++k)
-                if (k0 + k * G < g.parts) p.add(w[k].y, y[k], pa_weight(w[k].x, now, c));
+                p.add(w[k].y, y[k], pa_weight(w[k].x, now, c));
         }
 #pragma unroll
         for (int o = QW; o < 32; o <<= 1) {
@@ -115,10 +120,10 @@ __device__ __forceinline__ void merge_item(const PaArgs& a, const PaItem& g)
 }
 
 template <typename C, int HD, int ROWS, int TILES>
-__device__ __forceinline__ void merge_item(const PaArgs& a, const PaItem& g)
+__device__ __forceinline__ void merge_item(const PaArgs& a, const PaItem& g, int block, int blocks)
 {
-    if (g.parts <= 4) merge_item<C, HD, ROWS, TILES, 1>(a, g);
-    else merge_item<C, HD, ROWS, TILES, 4>(a, g);
+    if (g.parts <= 4) merge_item<C, HD, ROWS, TILES, 1>(a, g, block, blocks);
+    else merge_item<C, HD, ROWS, TILES, 4>(a, g, block, blocks);
 }
 
 template <typename C, int HD>
@@ -126,18 +131,19 @@ __global__ void __launch_bounds__(kPmThreads) paged_merge_kernel(const __grid_co
 {
     pdl_trigger();
     pdl_wait();
-    const bool is_few = blockIdx.z == 1 || !tiles.items;
+    const int few_blocks = few.items ? kPmFewBlocks : 0, block = blockIdx.y;
+    const bool is_few = block < few_blocks;
     const PaArgs& a = is_few ? few : tiles;
     const PaItem g = a.items[blockIdx.x];
-    if (blockIdx.z == 0) {                            // rows behind the last sequence's are padding: zeros
+    {                                                 // rows behind the last sequence's are padding: zeros
         const size_t row16 = (size_t)a.hq * HD / 8, n = row16 * a.b.rows, threads = (size_t)gridDim.x * gridDim.y * kPmThreads;
         const size_t first = row16 * max(a.b.cu_rows[a.b.seqs], 0);
         for (size_t i = first + (blockIdx.y * gridDim.x + blockIdx.x) * kPmThreads + threadIdx.x; i < n; i += threads)
             reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
     }
     if (g.parts < 2) return;
-    if (is_few) merge_item<C, HD, kPaFew, 1>(a, g);
-    else merge_item<C, HD, kPaRows, 2>(a, g);
+    if (is_few) merge_item<C, HD, kPaFew, 1>(a, g, block, kPmFewBlocks);
+    else merge_item<C, HD, kPaRows, 2>(a, g, block - few_blocks, kPmBlocks);
 }
 
 template <typename C>
@@ -151,7 +157,7 @@ int pa_launch_merge(const PaArgs* tiles, const PaArgs* few, int ctas, cudaStream
 {
     const PaArgs none{};
     const PaArgs& a = tiles ? *tiles : *few;
-    const dim3 grid(ctas, tiles ? kPmBlocks : kPmFewBlocks, tiles && few ? 2 : 1);
+    const dim3 grid(ctas, (tiles ? kPmBlocks : 0) + (few ? kPmFewBlocks : 0));
     return a.b.dtype == EXL3_F16 ? launch_merge<__half>(tiles ? *tiles : none, few ? *few : none, a.b.head_dim, grid, s)
                                  : launch_merge<__nv_bfloat16>(tiles ? *tiles : none, few ? *few : none, a.b.head_dim, grid, s);
 }
