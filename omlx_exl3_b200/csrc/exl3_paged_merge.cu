@@ -1,8 +1,8 @@
 // Merges the partial results of paged-attention items that were cut between CTAs, in CTA order:
 //   m = max m_k, out = sum_k exp2((m_k - m) c) O_k / sum_k exp2((m_k - m) c) l_k.
 //
-// grid (CTAs of the attention kernels, blocks of an item of few rows, then of one of tiles): block x looks at the item that started in CTA x's share.
-// (One CTA, the last to finish its part, merging alone was measured first: 40 rows of 33 parts are 0.7 MB, 25 us for one
+// grid (CTAs of the attention kernels, blocks of an item of few rows, then of one of tiles): block x looks at the item
+// that started in CTA x's share. (One CTA, the last to finish its part, merging alone was measured first: 40 rows of 33 parts are 0.7 MB, 25 us for one
 // SM.) The time is L2 latency, so a quad's parts are loaded four at a time, and by four threads where there are many.
 #include <cuda_runtime.h>
 
