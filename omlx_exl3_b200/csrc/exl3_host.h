@@ -28,7 +28,8 @@ inline int launch_status()
 // kernel in the stream is still running; it runs its independent prologue (the GEMV's first weight
 // loads), then waits in griddepcontrol.wait until the previous kernel has completed and its writes
 // are visible. Every kernel of this library that is launched this way makes that wait before it
-// touches anything the previous kernel may write or read.
+// touches anything the previous kernel may write or read (or, where the previous kernel lets it start only
+// after its own wait and shares no data with it, before it ends).
 inline bool pdl_enabled()
 {
     static int v = -1;
