@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     uint64_t* s_full = q_empty + 1;                   // [2][2] half of S of the slot is complete (and that half's P V before it)
     uint64_t* p_full = s_full + 4;                    // [2][2] half of P of the slot is written
     uint64_t* pv_done = p_full + 4;                   // [2] P V of the first half of the slot's step is complete
-    uint64_t* v_dirty = pv_done + 2;                   // the item's last V tile has landed and reaches past the sequence's end
+    uint64_t* v_dirty = pv_done + 2;                   // both issuing warps have taken the item's last V tile, which reaches past the end
     uint64_t* v_clean = v_dirty + 1;                  // it is zero there
     uint64_t* o_full = v_clean + 1;                   // [2] the slot's accumulator is complete
     uint64_t* o_empty = o_full + 2;                   // [2] it has been read
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         }
         mbar_init(q_full, 1);
         mbar_init(q_empty, 2 + 8);
-        mbar_init(v_dirty, 1);
+        mbar_init(v_dirty, 2);
         mbar_init(v_clean, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[2 * i], 1);
@@ -324,7 +324,8 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         // Between the MMAs of a step lie waits and commits of some hundred cycles in the issuing warp; with a warp per slot
         // they pass while the other slot's MMAs run. Each whole warp runs this and one elected lane issues, so that operands
         // come from uniform registers. Both warps see every tile of the ring land and release it (the tiles of the other
-        // slot at once), so neither can fall a round behind.
+        // slot at once), so neither can fall a round behind on the ring. Nor on a tile's cleaning: it begins when both have asked
+        // for it, so a warp without a step in a short item is past that item's v_clean before the next item's can complete.
         constexpr uint32_t idesc_s = pa_idesc<C>(kPaStep / 2, false), idesc_o = pa_idesc<C>(HD, true);
         const int slot = warp == 11;
         const uint32_t leader = elect_one();
@@ -400,7 +401,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                 uint32_t k = 0;
                 if (more) k = take();
                 if (m + 1 == n && dirty) {                             // warp 10 cleans it, once per such item
-                    if (lane == 0 && (dual ? slot == 0 : mine)) mbar_arrive(v_dirty);
+                    if (lane == 0) mbar_arrive(v_dirty);
                     wait(v_clean, n_clean++ & 1);
                 }
                 if (mine) {
