@@ -356,14 +356,15 @@ EXL3_API int exl3_peer_status(const exl3_peer_group* g, uint32_t* status);
  * whose cache belongs to oMLX and attention to the model library).
  *
  * k_pages / v_pages: (num_pages, hkv, page_size, head_dim), fp16 or bf16 (dtype), contiguous, 16-byte
- * aligned. Sequence s feeds rows cu_rows[s] .. cu_rows[s + 1] - 1 of a call (cu_rows[0] = 0,
+ * aligned. Sequence s feeds rows cu_rows[s] .. cu_rows[s + 1] - 1 of a call (0 <= cu_rows[0] <= .. <=
  * cu_rows[seqs] <= rows) and holds lens[s] positions once they are appended: its row i is at position
  * lens[s] - (cu_rows[s + 1] - cu_rows[s]) + i. Position p lives in page page_table[s][p / page_size].
- * A row at a negative position, or behind the last sequence's, is padding: nothing is appended for it and its
- * output is zero. All
+ * A row at a negative position, before the first sequence's or behind the last one's, is padding: nothing is
+ * appended for it and its output is zero. All
  * tables are int32 on the device and read by the kernels alone (a captured graph follows their contents).
  * What they name outside the pool, the page table or the rotation table is left out and sets bit 8 of
- * *status; a pipeline wait that gave up sets bit 1.
+ * *status; so does a cu_rows that falls or leaves 0 .. rows, for which attention computes nothing and gives
+ * zeros. A pipeline wait that gave up sets bit 1.
  */
 typedef struct exl3_paged_desc {
     void* k_pages;

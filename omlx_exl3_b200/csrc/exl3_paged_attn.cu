@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                 pg2 = pg3;
             }
         }
-        if (lane == 0) pa_record(a, n_seg > 0, g, n_seg > 0 ? min(2 * tokens, g.rows - by_grp(a, g.p0)) * a.grp : 0, tokens * a.grp);
+        if (lane == 0) pa_record(a, sched.bad, n_seg > 0, g, n_seg > 0 ? min(2 * tokens, g.rows - by_grp(a, g.p0)) * a.grp : 0, tokens * a.grp);
         // nothing of this CTA may still be landing when it exits
         for (uint32_t i = it > (uint32_t)P::kStages ? it - P::kStages : 0; i < it; ++i)
             if (!pa_wait(&full[i % P::kStages], (i / P::kStages) & 1, kPaExitNs)) ok = false;

@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(32 * kPfWarps, 1) paged_few_kernel(const __gri
             __syncthreads();
         }
     }
-    if (threadIdx.x == 0) pa_record(a, any, g, any ? min(8 * NQ, g.rows * a.grp - g.p0) : 0, 8 * NQ);   // g: the last segment
+    if (threadIdx.x == 0) pa_record(a, sched.bad, any, g, any ? min(8 * NQ, g.rows * a.grp - g.p0) : 0, 8 * NQ);   // g: the last segment
     cp_async_wait<0>();
     if (a.behind) pdl_wait();                         // so that the merge, which waits for this kernel, finds the tiles' parts too
 }

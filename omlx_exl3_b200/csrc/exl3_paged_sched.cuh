@@ -38,7 +38,7 @@ struct PaArgs {
     int lo, hi;                                       // sequences of lo < rows * grp <= hi are this kernel's
 };
 
-// An item whose parts are to be merged; parts 0: none.
+// An item whose parts are to be merged; parts 0: none; -1: cu_rows is no list of rows, and nothing was computed.
 struct PaItem {
     int parts, c0, h, start, p0, used, gap, pad;      // first packed row, packed rows; rows of tile 1 follow `gap` after p0
 };
@@ -67,6 +67,7 @@ struct PaSched {
     int share, begin, until;                          // a share's length, the current item's place in the list, this share's end
     int s, h, t, j, cap;
     int rows, len;                                    // of sequence s
+    bool bad;                                         // cu_rows falls somewhere, or leaves 0 .. b.rows
 
     __device__ __forceinline__ explicit PaSched(const PaArgs& args) : a(args) {}
 
@@ -82,15 +83,15 @@ struct PaSched {
     // Rows and length of sequence q: a length that could not be one is taken as the nearest that could.
     __device__ __forceinline__ void load(int q, int& r, int& n) const
     {
-        r = a.b.cu_rows[q + 1] - a.b.cu_rows[q];
-        r = max(0, min(r, a.b.rows));
+        r = a.b.cu_rows[q + 1] - a.b.cu_rows[q];      // start() has seen that this lies in 0 .. b.rows
         n = max(0, min(a.b.lens[q], cap + a.b.rows));
     }
 
-    // Length of sequence q in the list, for one kv head.
+    // Length of sequence q in the list, for one kv head; -1: its rows are out of order or out of range.
     __device__ __forceinline__ int head_length(int q) const
     {
         if (q >= a.b.seqs) return 0;
+        if (a.b.cu_rows[q] < 0 || a.b.cu_rows[q + 1] < a.b.cu_rows[q] || a.b.cu_rows[q + 1] > a.b.rows) return -1;
         int r, n, sum = 0;
         load(q, r, n);
         if (!takes(r)) return 0;
@@ -98,18 +99,23 @@ struct PaSched {
         return sum;
     }
 
-    // All lanes of the warp. This CTA's share of the list, and where it starts.
+    // All lanes of the warp. This CTA's share of the list, and where it starts. Rows that rise from sequence to sequence within
+    // 0 .. b.rows are no more than b.rows in all, which is what the list's 32 bits and every row index below rest on; any other
+    // cu_rows gives an empty list.
     __device__ __forceinline__ void start(int cta, int grid, int lane)
     {
         cap = a.b.table_cols * a.b.page_size;
         int first = 0, total = 0;                     // first: this lane's part of the first 32 sequences
+        bad = false;
         for (int q0 = 0; q0 < a.b.seqs; q0 += 32) {
             const int n = head_length(q0 + lane);
             if (q0 == 0) first = n;
+            bad |= __any_sync(0xffffffffu, n < 0);
             total += __reduce_add_sync(0xffffffffu, n) * a.b.hkv;
         }
         s = h = t = j = 0;
         begin = until = 0;
+        if (bad) total = 0;
         share = (total + grid - 1) / grid;
         const int u = cta * share;
         if (u >= total) return;
@@ -205,9 +211,13 @@ __device__ __forceinline__ uint8_t* pa_part(uint8_t* parts, int c0, int cta, int
 }
 
 // After its last segment g (any == false: it had none) a CTA records the item that it starts and does not finish.
-__device__ __forceinline__ void pa_record(const PaArgs& a, bool any, const PaSeg& g, int used, int gap)
+__device__ __forceinline__ void pa_record(const PaArgs& a, bool bad, bool any, const PaSeg& g, int used, int gap)
 {
     PaItem it{};
+    if (bad) {
+        it.parts = -1;
+        if (blockIdx.x == 0) atomicOr(a.status, kStatusPagedRange);
+    }
     if (any && g.j0 == 0 && g.j1 < g.units) {
         it.parts = g.c1 - g.c0 + 1;
         it.c0 = g.c0;

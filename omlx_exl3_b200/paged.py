@@ -10,12 +10,13 @@ is the part of a server that sits between the EXL3 projections:
 
 A batch is cu_rows (seqs + 1), lens (seqs) and page_table (seqs, cols), all int32 on the device: sequence s feeds
 rows cu_rows[s] .. cu_rows[s + 1] - 1 and holds lens[s] positions once they are appended, so its row i is at
-position lens[s] - rows[s] + i; position p lives in page page_table[s, p // page_size]. Rows at negative positions
-and rows from cu_rows[seqs] on are padding: nothing is appended and the output is zero (a captured graph's unused
-slots have no rows, or lens 0). The kernels read the tables themselves, so no call waits for the host and a captured graph follows their contents.
+position lens[s] - rows[s] + i; position p lives in page page_table[s, p // page_size]. Rows at negative positions,
+rows before cu_rows[0] and rows from cu_rows[seqs] on are padding: nothing is appended and the output is zero (a captured
+graph's unused slots have no rows, or lens 0). The kernels read the tables themselves, so no call waits for the host and a captured graph
+follows their contents.
 
-Calls run on the current stream. Tables that name something outside the pool set a bit in a per-device status
-word, as a pipeline wait that gave up does: check_paged_status() raises on it.
+Calls run on the current stream. Tables that name something outside the pool, or a cu_rows that falls or passes the
+call's rows, set a bit in a per-device status word, as a pipeline wait that gave up does: check_paged_status() raises on it.
 """
 from __future__ import annotations
 
