@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(32 * kDecideWarps) verify_decide_kernel(const 
                 if (greedy) {
                     p = in && v.token == v.p.first && v.p.inv > 0.f ? 1.f : 0.f;
                 } else {
-                    if (in) p = ex2((xt - v.p.m) * c) * v.p.inv;
+                    if (in && v.p.inv > 0.f) p = ex2((xt - v.p.m) * c) * v.p.inv;       // a NaN logit is in a row without probabilities
                     if (two) q = in ? ex2((xd - v.q.m) * c) * v.q.inv : 0.f;
                 }
                 v.prob = q > 0.f ? fminf(p / q, 1.f) : (p > 0.f ? 1.f : 0.f);
