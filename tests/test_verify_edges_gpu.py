@@ -32,3 +32,43 @@ def test_rows_that_are_not_numbers_accept_nothing(cuda, dtype, n, temp, dist):
     got = _check(cuda, target, tokens, cu, u, noise, 3, draft if dist else None, t)
     assert got[1].tolist()[:3] == [1, 1, 1] and got[0][:3, 0].tolist() == [-1] * 3
     assert got[2][[0, 3, 6]].tolist() == [0.0] * 3
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("value", [41.0, 47.0, 55.0])
+@pytest.mark.parametrize("seqs", [1, 40])                              # wide CTAs, and narrow ones
+@pytest.mark.parametrize("n,off", [(8, 0), (1 << 12, 0), (1 << 12, 1), (1 << 15, 8)])
+def test_equal_weights_go_to_the_first(cuda, dtype, value, seqs, n, off):
+    """Equal logits and equal noise: all quotients are one number, so the first column wins, whichever thread, vector or
+    scalar path it falls to; after a rejection the first that is not the draft (one-hot q) or that p - q leaves."""
+    wide = torch.zeros((2 * seqs, n + 16), dtype=dtype, device=cuda)
+    target = wide[:, off:off + n]
+    noise = torch.full((seqs, n + 16), value, device=cuda)[:, off:off + n]
+    cu = list(range(0, 2 * seqs + 1, 2))
+    tokens, u = torch.zeros(seqs, dtype=torch.int64), torch.full((seqs,), 0.9999)
+    ones = torch.arange(seqs + 1).tolist()
+    out, count, _ = _verify(cuda, target[:seqs], tokens[:0], ones, u[:0], noise, 0)
+    assert not out.any() and (count == 1).all()
+    draft = torch.zeros((seqs, n), dtype=dtype)
+    draft[:, 0] = 2.0                                                  # q is above p there and below it, alike, elsewhere
+    for d in (None, draft):
+        out, count, prob = _verify(cuda, target, tokens, cu, u, noise, 1, d)
+        assert (prob < 0.9999).all() and (count == 1).all() and (out[:, 0] == 1).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("seqs", [18, 70])                             # wide CTAs, and narrow ones
+@pytest.mark.parametrize("off", [0, 3])
+def test_close_races_go_by_the_rounded_quotient(cuda, dtype, seqs, off):
+    """p is 2^-12 in every column, exactly, and a sequence's noise takes three neighbouring fp32 numbers, whose quotients are equal
+    or one unit apart: the first column with the largest fp32 quotient wins in every layout."""
+    n = 1 << 12
+    g = torch.Generator().manual_seed(seqs)
+    noise = 1.5 + 0.45 * torch.rand((seqs, 1), generator=g) + torch.randint(0, 3, (seqs, n), generator=g) * 2.0 ** -23
+    want = 2.0 ** -12 / noise
+    want = (want == want.amax(1, keepdim=True)).int().argmax(1)
+    wide = torch.zeros((seqs, n + 8), device=cuda)
+    wide[:, off:off + n] = noise.to(cuda)
+    target = torch.zeros((seqs, n), dtype=dtype)
+    out, _, _ = _verify(cuda, target, torch.zeros(0, dtype=torch.int64), list(range(seqs + 1)), torch.zeros(0), wide[:, off:off + n], 0)
+    assert torch.equal(out[:, 0], want)
