@@ -414,7 +414,8 @@ EXL3_API int exl3_paged_attn(const exl3_paged_desc* batch, const void* q, long l
  *   first rejected draft (p where that is zero everywhere) or p at the row after the last accepted one.
  * noise: positive, exponentially distributed (that makes the race a draw from w). tokens_out (seqs,
  * max_drafts + 1): the accepted drafts, the next token, then -1; count = accepted + 1. A row whose logits
- * are all -inf (or not numbers) accepts nothing and gives token -1. Drafts past max_drafts are not looked at.
+ * are all -inf, or that has a NaN or (T > 0) a +inf, has no probabilities: it accepts nothing and gives token -1. At T = 0 a
+ * +inf is the largest logit. Drafts past max_drafts are not looked at.
  * target (rows, n) and draft (rows - seqs, n) in one dtype (fp16, bf16, fp32), rows ld elements apart;
  * temperature (seqs) may be null (1).
  */

@@ -17,6 +17,7 @@
 // sequence's statistics are known. One sequence of 4 rows: 12.5 us, two launches and two rounds of loads.
 #include <cuda_runtime.h>
 
+#include <cfloat>
 #include <type_traits>
 
 #include "exl3_b200.h"
@@ -153,7 +154,8 @@ __global__ void __launch_bounds__(kStatThreads, 8) verify_stats_kernel(const Ver
     m = sv[lane & (kStatWarps - 1)];
 #pragma unroll
     for (int o = kStatWarps / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base = m == -INFINITY ? 0.f : m, c = exponent_scale(temp, greedy);
+    // relative to the largest finite number where the maximum is +inf: the sum is inf then, and NaN only where a logit is
+    const float base = m == -INFINITY ? 0.f : fminf(m, FLT_MAX), c = exponent_scale(temp, greedy);
     // the maximum is taken off before scaling: the type's lowest value times 1 / T would overflow
     const uint64_t c2 = f2(c, c), zero = f2(0.f, 0.f), off = f2(-base, -base);
     uint64_t s2 = f2(ex2((xh - base) * c), 0.f);
@@ -198,7 +200,8 @@ __global__ void __launch_bounds__(kStatThreads, 8) verify_stats_kernel(const Ver
             sum += sv[k];
             col = min(col, si[k]);
         }
-        a.stats[blockIdx.x] = make_float4(m, sum, __int_as_float(col), 0.f);
+        // at T = 0 the sum only tells whether the row has an answer: a +inf is a maximum like any other
+        a.stats[blockIdx.x] = make_float4(m, greedy && sum > 0.f ? 1.f : sum, __int_as_float(col), 0.f);
     }
 }
 
@@ -210,10 +213,11 @@ struct RowStat {
 };
 
 // Two sums of exp relative to their own maxima, relative to the larger one. A part of -inf alone has sum 0 (or NaN, which
-// stays: its row has no probabilities).
+// stays: its row has no probabilities); one whose maximum is the larger, +inf too, passes as it is.
 __device__ __forceinline__ float joined(float s0, float m0, float s1, float m1, float now, float c)
 {
-    return (m0 == -INFINITY ? s0 : s0 * ex2((m0 - now) * c)) + (m1 == -INFINITY ? s1 : s1 * ex2((m1 - now) * c));
+    auto rel = [&](float s, float m) { return m == -INFINITY || m == now ? s : s * ex2((m - now) * c); };
+    return rel(s0, m0) + rel(s1, m1);
 }
 
 struct PartStat {                                     // of some of a row's chunks

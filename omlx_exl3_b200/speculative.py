@@ -24,6 +24,7 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, cu_ro
 
     A draft x stands while u < min(1, p(x) / q(x)); the next token is drawn from max(0, p - q) after a rejection, else
     from the last row's p, as the first largest w(v) / noise[s, v]. tokens holds the accepted drafts, the next token,
-    then -1; count is the accepted drafts + 1. A row without any finite probability accepts nothing and gives -1.
+    then -1; count is the accepted drafts + 1. A row without any finite probability (all logits -inf, one of them NaN or, but
+    for T = 0, +inf) accepts nothing and gives -1.
     """
     return torch_calls().verify_drafts(target_logits, draft_tokens, cu_rows, u, noise, max_drafts, draft_logits, temperature)

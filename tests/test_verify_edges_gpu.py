@@ -72,3 +72,30 @@ def test_close_races_go_by_the_rounded_quotient(cuda, dtype, seqs, off):
     target = torch.zeros((seqs, n), dtype=dtype)
     out, _, _ = _verify(cuda, target, torch.zeros(0, dtype=torch.int64), list(range(seqs + 1)), torch.zeros(0), wide[:, off:off + n], 0)
     assert torch.equal(out[:, 0], want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [700, 40001])
+def test_greedy_takes_infinity_as_the_largest_logit(cuda, dtype, n):
+    """At T = 0 a token forced by +inf is the first maximum, alone or among others and beside -inf; a NaN in the row still means
+    that it has no answer. At other temperatures inf / inf is no probability."""
+    target, tokens, cu, u, noise, _, _ = _inputs([3, 2, 2, 1, 1], n, dtype, seed=n + 1)
+    u = torch.full_like(u, 0.999)
+    target[0, n - 1] = INF
+    tokens[0] = n - 1
+    target[1, [n // 2, n - 5]] = INF
+    tokens[1] = n - 5                                                  # not the first maximum
+    target[3] = -INF
+    target[3, n // 3] = INF
+    tokens[2] = n // 3
+    target[4, 5] = INF
+    target[5, [3, n - 2]] = INF
+    target[5, n // 2] = NAN
+    target[7] = INF
+    target[8, 1] = INF
+    temp = torch.tensor([0.0, 0.0, 0.0, 0.0, 1.0])
+    tokens[3] = 3
+    out, count, prob = _verify(cuda, target, tokens, cu, u, noise, 2, None, temp)
+    assert prob.tolist() == [1.0, 0.0, 1.0, 0.0] and count.tolist() == [2, 2, 1, 1, 1]
+    assert out[0].tolist() == [n - 1, n // 2, -1] and out[1].tolist() == [n // 3, 5, -1]
+    assert out[2:, 0].tolist() == [-1, 0, -1]
