@@ -415,7 +415,8 @@ EXL3_API int exl3_paged_attn(const exl3_paged_desc* batch, const void* q, long l
  * noise: positive, exponentially distributed (that makes the race a draw from w). tokens_out (seqs,
  * max_drafts + 1): the accepted drafts, the next token, then -1; count = accepted + 1. A row whose logits
  * are all -inf, or that has a NaN or (T > 0) a +inf, has no probabilities: it accepts nothing and gives token -1. At T = 0 a
- * +inf is the largest logit. Drafts past max_drafts are not looked at.
+ * +inf is the largest logit. Drafts past max_drafts are not looked at. A sequence whose cu_rows leave 0 .. rows or name
+ * no row gives count 0 and tokens -1, and a draft that no sequence judges has accept_prob 0.
  * target (rows, n) and draft (rows - seqs, n) in one dtype (fp16, bf16, fp32), rows ld elements apart;
  * temperature (seqs) may be null (1).
  */

@@ -106,6 +106,8 @@ __global__ void __launch_bounds__(kStatThreads, 8) verify_stats_kernel(const Ver
                           : static_cast<const T*>(a.target) + r * a.target_ld;
     const int head = min(a.n, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
     const int first = head + chunk * (kStatThreads * N * VEC) + tid * VEC;
+    // the decision writes those of the drafts that a sequence judges; a draft that none does (a cu_rows that is no list) has 0
+    if (tid == 0 && chunk == 0 && r < a.rows - a.seqs) a.prob[r] = 0.f;
     const uint32_t none = lowest_word<T>();
     uint4 w[N];
     auto fetch = [&]() {

@@ -99,3 +99,18 @@ def test_greedy_takes_infinity_as_the_largest_logit(cuda, dtype, n):
     assert prob.tolist() == [1.0, 0.0, 1.0, 0.0] and count.tolist() == [2, 2, 1, 1, 1]
     assert out[0].tolist() == [n - 1, n // 2, -1] and out[1].tolist() == [n // 3, 5, -1]
     assert out[2:, 0].tolist() == [-1, 0, -1]
+
+
+@pytest.mark.parametrize("dist", [True, False])
+def test_rows_that_no_table_claims(cuda, dist):
+    """cu_rows past the rows, or going back: such a sequence gives count 0 and no tokens, and drafts that none judged have
+    acceptance 0, not what the memory held."""
+    target, tokens, _, u, noise, draft, _ = _inputs([1, 4], 300, torch.float16, seed=3)
+    u = torch.zeros_like(u)
+    for bad in ([0, 1, 9], [0, 1, 0], [0, 1, 1], [0, 1, -4], [0, 1, 2 ** 31 - 1]):
+        for _ in range(3):                                             # memory that the outputs may be given next
+            junk = [torch.full((3,), 7.0, device=cuda) for _ in range(64)]
+            del junk
+            out, count, prob = _verify(cuda, target, tokens, bad, u, noise, 3, draft if dist else None)
+            assert count.tolist() == [1, 0] and out[1].tolist() == [-1] * 4 and out[0, 0] >= 0
+            assert prob.tolist() == [0.0] * 3
