@@ -378,6 +378,9 @@ typedef struct exl3_paged_desc {
     int32_t dtype;                 /* EXL3_F16 or EXL3_BF16 */
 } exl3_paged_desc;
 
+/* *taken = *status (both on the device), which becomes 0 in the same step: no bit that another stream's call sets is lost. */
+EXL3_API int exl3_paged_status_take(uint32_t* status, uint32_t* taken, void* stream);
+
 /*
  * After the q/k/v projections: per-head RMSNorm of q and k (q_norm_w / k_norm_w (head_dim) in in_dtype, or
  * null for none), rotate-half rotary embedding of the first 2 * rope_half elements (cos / sin fp32

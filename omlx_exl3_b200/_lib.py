@@ -109,6 +109,7 @@ SIGNATURES = {
     "exl3_gemv_swiglu": (_I, [ctypes.POINTER(GemvDesc), _P, _I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "exl3_gemv_swiglu_peer": (_I, [ctypes.POINTER(GemvDesc), _P, _I, _P, _P, _P, _P, _P, _P, _SZ,
                                    ctypes.POINTER(PeerGroupDesc), _I, _P]),
+    "exl3_paged_status_take": (_I, [_P, _P, _P]),
     "exl3_paged_qkv_post": (_I, [_PAGED, _P, _P, _P, _LL, _LL, _LL, _I, _I, _P, _P, _F, _P, _P, _I, _I, _P, _P, _P]),
     "exl3_paged_attn_workspace": (_I, [_PAGED, _I, ctypes.POINTER(_SZ)]),
     "exl3_paged_attn": (_I, [_PAGED, _P, _LL, _I, _F, _I, _P, _P, _SZ, _P, _P]),

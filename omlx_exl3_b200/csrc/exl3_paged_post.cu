@@ -162,6 +162,9 @@ __global__ void __launch_bounds__(128, 6) paged_post_kernel(const PagedPostArgs 
     }
 }
 
+// Reads and clears in one step, so that a bit set meanwhile is in this reading or the next.
+__global__ void paged_status_take_kernel(uint32_t* status, uint32_t* taken) { *taken = atomicExch(status, 0u); }
+
 template <typename T, typename C, bool VEC>
 static int launch_post(const PagedPostArgs& a, dim3 grid, cudaStream_t s)
 {
@@ -192,6 +195,15 @@ int exl3_check_paged(const exl3_paged_desc* b)
         !aligned(b->lens, 4))
         return EXL3_E_ALIGN;
     return EXL3_OK;
+}
+
+extern "C" int exl3_paged_status_take(uint32_t* status, uint32_t* taken, void* stream)
+{
+    if (!status || !taken) return EXL3_E_NULL;
+    if (!aligned(status, 4) || !aligned(taken, 4)) return EXL3_E_ALIGN;
+    if (int e = check_device()) return e;
+    paged_status_take_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(status, taken);
+    return launch_status();
 }
 
 extern "C" int exl3_paged_qkv_post(const exl3_paged_desc* batch, const void* q, const void* k, const void* v,

@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -76,7 +77,9 @@ uint32_t* status_word(const Tensor& like)
     const auto it = words.find(like.get_device());
     if (it != words.end()) return reinterpret_cast<uint32_t*>(it->second.data_ptr());
     TORCH_CHECK(!capturing(), "call a paged kernel once on this device before capturing it in a graph");
+    const c10::InferenceMode plain(false);            // whoever makes the first call
     Tensor word = at::zeros({4}, like.options().dtype(at::kInt));
+    at::cuda::getCurrentCUDAStream().synchronize();   // zero before a call on any other stream may set a bit
     words[like.get_device()] = word;
     return reinterpret_cast<uint32_t*>(word.data_ptr());
 }
@@ -293,6 +296,23 @@ PyObject* verify_drafts(PyObject*, PyObject* const* arg, Py_ssize_t n_arg)
     END_HANDLE_TH_ERRORS
 }
 
+// take_status(device index) -> the device's status word as a tensor of its own, the word cleared; None where no paged kernel has run
+PyObject* take_status(PyObject*, PyObject* const* arg, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    NEED_TYPE(n == 1, "take_status takes one argument");
+    auto& words = status_words();
+    const auto it = words.find((int)integer(arg[0], "device"));
+    if (it == words.end()) Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(it->second.device());
+    Tensor taken = at::empty({1}, it->second.options());
+    raise_status(exl3_paged_status_take(reinterpret_cast<uint32_t*>(it->second.data_ptr()), reinterpret_cast<uint32_t*>(taken.data_ptr()),
+                                        at::cuda::getCurrentCUDAStream().stream()),
+                 "exl3_paged_status_take");
+    return THPVariable_Wrap(taken);
+    END_HANDLE_TH_ERRORS
+}
+
 // status(device index) -> the device's status word as a tensor, or None where no paged kernel has run
 PyObject* status(PyObject*, PyObject* const* arg, Py_ssize_t n)
 {
@@ -306,7 +326,8 @@ PyObject* status(PyObject*, PyObject* const* arg, Py_ssize_t n)
 }
 
 #define CALL(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {CALL(paged_qkv_post), CALL(paged_attn), CALL(verify_drafts), CALL(status), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {CALL(paged_qkv_post), CALL(paged_attn), CALL(verify_drafts), CALL(status), CALL(take_status),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_exl3_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -30,17 +30,25 @@ def _device_index(device: torch.device | None) -> int:
 
 
 def paged_status(device: torch.device | None = None) -> int:
-    """The device's status word of the paged kernels (0: nothing was out of range, no wait gave up); synchronises."""
-    word = torch_calls().status(_device_index(device))
-    return 0 if word is None else int(word[0].item())
+    """The device's status word of the paged kernels (0: nothing was out of range, no wait gave up). Waits for all of the
+    device's streams."""
+    index = _device_index(device)
+    word = torch_calls().status(index)
+    if word is None:
+        return 0
+    torch.cuda.synchronize(index)
+    return int(word[0].item())
 
 
 def check_paged_status(device: torch.device | None = None) -> None:
     """Raise RuntimeError if a paged kernel on `device` met a page, position or wait it could not serve, and clear
-    the word. Synchronises."""
-    value = paged_status(device)
+    the word. Waits for all of the device's streams."""
+    index = _device_index(device)
+    if torch_calls().status(index) is None:
+        return
+    torch.cuda.synchronize(index)
+    value = int(torch_calls().take_status(index).item())
     if value:
-        torch_calls().status(_device_index(device)).zero_()
         what = [t for bit, t in ((8, "a table names a page or position outside its range"),
                                  (1, "a pipeline wait timed out")) if value & bit]
         raise RuntimeError(f"paged kernels: {'; '.join(what) or 'error'} (status 0x{value:x}); the outputs of the "
