@@ -72,7 +72,8 @@ class PagedEngine:
         return torch.tensor(values, dtype=dtype).pin_memory().to(self.device, non_blocking=True)
 
     def step(self) -> dict:
-        """One batch; returns the new tokens of the sequences that have some (finished ones leave the engine)."""
+        """One batch; returns the new tokens of the sequences that have some (finished ones leave the engine). A step that raises
+        changes nothing: the next one feeds the same rows."""
         feeds, room = [], self.chunk
         for key, s in self._seqs.items():
             have = self.cache.length(key)
@@ -88,11 +89,21 @@ class PagedEngine:
             feeds.append((key, s, [s.tokens[-1]] + drafts, drafts, True))
         if not feeds:
             return {}
+        judged = [(key, s, drafts) for key, s, _, drafts, wanted in feeds if wanted]
         lengths = {key: self.cache.length(key) for key, *_ in feeds}
+        try:
+            picked = self._run(feeds, judged)
+        except BaseException:                                       # as before the step: its rows leave the cache again
+            for key, length in lengths.items():
+                self.cache.truncate(key, length)
+            raise
+        return self._keep(judged, picked, lengths)
+
+    def _run(self, feeds: list, judged: list) -> list:
+        """The batch through the model and the verification; for each judged sequence its tokens and their count."""
         batch = self.cache.extend([(key, len(rows)) for key, _, rows, _, _ in feeds])
         tokens = self._upload([t for _, _, rows, _, _ in feeds for t in rows], torch.int64)
         # rows whose logits are wanted: a decoding sequence's all, a finished prompt's last
-        judged = [(key, s, drafts) for key, s, _, drafts, wanted in feeds if wanted]
         at, rows, cu = 0, [], [0]
         for _, _, fed, drafts, wanted in feeds:
             at += len(fed)
@@ -100,16 +111,14 @@ class PagedEngine:
                 rows += range(at - len(drafts) - 1, at)
                 cu.append(len(rows))
         logits = self.model.forward_paged(tokens, self.cache, batch, self._upload(rows, torch.int64) if rows else None)
-        out = {}
-        if judged:
-            out = self._verify(self.model.gather_logits(logits), judged, cu, lengths)
+        picked = self._verify(self.model.gather_logits(logits), judged, cu) if judged else []
         self._unchecked += 1
         if self.check_every and self._unchecked >= self.check_every:
             self._unchecked = 0
             check_paged_status(self.device)
-        return out
+        return picked
 
-    def _verify(self, logits: torch.Tensor, judged: list, cu: list[int], lengths: dict) -> dict:
+    def _verify(self, logits: torch.Tensor, judged: list, cu: list[int]) -> list:
         drafts = [t for _, _, d in judged for t in d]
         most = max(len(d) for _, _, d in judged)
         n, vocab = len(judged), logits.shape[1]
@@ -117,7 +126,10 @@ class PagedEngine:
         u = torch.rand(len(drafts), device=self.device, generator=self._gen)
         picked, count, _ = verify_drafts(logits, self._upload(drafts, torch.int64), self._upload(cu, torch.int32), u, noise, most,
                                          temperature=self._upload([s.temperature for _, s, _ in judged], torch.float32))
-        picked = torch.cat([picked, count[:, None]], 1).tolist()    # the step's one wait for the GPU
+        return torch.cat([picked, count[:, None]], 1).tolist()      # the step's one wait for the GPU
+
+    def _keep(self, judged: list, picked: list, lengths: dict) -> dict:
+        """Take a finished step's tokens over, and what was not accepted out of the cache."""
         out = {}
         for (key, s, d), row in zip(judged, picked):
             got = row[:row[-1]]

@@ -1,0 +1,86 @@
+"""CPU: the engine's steps over a stand-in for the decoder, undisturbed and disturbed."""
+import pytest
+
+from omlx_exl3_b200 import serving
+from omlx_exl3_b200.serving import PagedEngine
+from serving_util import HistoryModel, greedy_text, on_cpu
+
+PROMPTS = [[1, 2, 3, 1, 2, 3, 1], list(range(30, 70)), [5], [9, 9, 9, 9]]
+
+
+@pytest.fixture(autouse=True)
+def _cpu(monkeypatch):
+    on_cpu(monkeypatch)
+
+
+def _run(engine, out=None):
+    """Steps until nothing runs; the tokens of each key."""
+    out = {} if out is None else out
+    for _ in range(2000):
+        if not engine.running:
+            return out
+        for key, tokens in engine.step().items():
+            out.setdefault(key, []).extend(tokens)
+    raise AssertionError("the engine does not finish")
+
+
+def _state(engine):
+    return ({k: engine.cache.length(k) for k in engine._seqs}, engine.cache.free_pages,
+            {k: (list(s.tokens), list(s.new)) for k, s in engine._seqs.items()})
+
+
+def _mostly_right(tokens, most):
+    """Drafts of the true text, some of them wrong."""
+    want = greedy_text(tokens, most)
+    return [t if (len(tokens) + i) % 3 else (t + 1) % 97 for i, t in enumerate(want)]
+
+
+@pytest.mark.parametrize("chunk,drafts", [(512, 0), (7, 4), (1, 2)])
+def test_undisturbed(chunk, drafts):
+    engine = PagedEngine(HistoryModel(), 40, 16, chunk=chunk, max_drafts=drafts, propose=_mostly_right)
+    assert engine.generate(PROMPTS, 13) == [greedy_text(p, 13) for p in PROMPTS]
+    assert engine.cache.free_pages == 40
+
+
+class Broken(Exception):
+    pass
+
+
+@pytest.mark.parametrize("part", ["forward", "gather", "verify", "status", "noise"])
+@pytest.mark.parametrize("when", [1, 2, 4])
+def test_a_step_that_raises_changes_nothing(monkeypatch, part, when):
+    """Whatever fails within a step, sequences and pages are as before it, and the next steps write the undisturbed text."""
+    calls = []
+
+    def once(result):
+        def f(*args, **kw):
+            calls.append(1)
+            if len(calls) == when:
+                raise Broken
+            return result(*args, **kw)
+        return f
+    model = HistoryModel()
+    engine = PagedEngine(model, 40, 16, chunk=16, max_drafts=3, propose=_mostly_right, check_every=1)
+    if part == "forward":
+        model.fail = once(lambda step: None)
+    elif part == "gather":
+        model.gather_logits = once(lambda x: x)
+    elif part == "noise":
+        monkeypatch.setattr(serving.torch, "rand", once(serving.torch.rand))
+    else:
+        name = {"verify": "verify_drafts", "status": "check_paged_status"}[part]
+        monkeypatch.setattr(serving, name, once(getattr(serving, name)))
+    for i, p in enumerate(PROMPTS):
+        engine.add(i, p, 13)
+    out, before, raised = {}, None, 0
+    while engine.running:
+        before = _state(engine)
+        try:
+            for key, tokens in engine.step().items():
+                out.setdefault(key, []).extend(tokens)
+        except Broken:
+            raised += 1
+            assert _state(engine) == before
+    assert raised == 1
+    assert [out[i] for i in range(len(PROMPTS))] == [greedy_text(p, 13) for p in PROMPTS]
+    assert engine.cache.free_pages == 40
