@@ -53,6 +53,7 @@ class PagedEngine:
         self._gen = torch.Generator(device=self.device)
         self._gen.manual_seed(seed)
         self._seqs: dict = {}
+        self.failed: dict = {}                                      # sequences that left without an end, and why
         self.drafted = self.accepted = 0
 
     @property
@@ -66,6 +67,7 @@ class PagedEngine:
         if len(prompt) + max_new > self.model.cfg.max_position_embeddings:
             raise ValueError(f"{len(prompt)} + {max_new} tokens exceed max_position_embeddings")
         self.cache.add(key)
+        self.failed.pop(key, None)
         self._seqs[key] = _Sequence(list(prompt), len(prompt), max_new, float(temperature), frozenset(stop))
 
     def _upload(self, values: list, dtype) -> torch.Tensor:
@@ -73,7 +75,8 @@ class PagedEngine:
 
     def step(self) -> dict:
         """One batch; returns the new tokens of the sequences that have some (finished ones leave the engine). A step that raises
-        changes nothing: the next one feeds the same rows."""
+        changes nothing: the next one feeds the same rows. A sequence for which the model gives no probabilities leaves too, and
+        `failed` names it."""
         feeds, room = [], self.chunk
         for key, s in self._seqs.items():
             have = self.cache.length(key)
@@ -133,20 +136,25 @@ class PagedEngine:
         out = {}
         for (key, s, d), row in zip(judged, picked):
             got = row[:row[-1]]
-            if got[-1] < 0:
-                raise RuntimeError(f"sequence {key!r}: the model gave no probabilities")
+            dead = got[-1] < 0                                      # no token after the drafts that stand
+            if dead:
+                got.pop()
             self.drafted += len(d)
-            self.accepted += len(got) - 1
-            if lengths[key] >= s.prompt:                            # its last token and the drafts that stand are cached
-                self.cache.truncate(key, lengths[key] + len(got))
+            self.accepted += len(got) - (not dead)
             end = next((i + 1 for i, t in enumerate(got) if t in s.stop), len(got))
             got = got[:min(end, s.max_new - len(s.new))]
             s.tokens += got
             s.new += got
-            out[key] = got
-            if len(s.new) >= s.max_new or got[-1] in s.stop:
+            if got:
+                out[key] = got
+            ended = len(s.new) >= s.max_new or (got and got[-1] in s.stop)
+            if dead and not ended:
+                self.failed[key] = "the model gave no probabilities"
+            if dead or ended:
                 self.cache.release(key)
                 del self._seqs[key]
+            elif lengths[key] >= s.prompt:                          # its last token and the drafts that stand stay cached
+                self.cache.truncate(key, lengths[key] + len(got))
         return out
 
     def generate(self, prompts: list[list[int]], max_new: int, temperature: float = 0.0, stop=()) -> list[list[int]]:
@@ -157,5 +165,8 @@ class PagedEngine:
         while self.running:
             for i, got in self.step().items():
                 done[i] += got
+            for i in done:
+                if i in self.failed:
+                    raise RuntimeError(f"prompt {i}: {self.failed[i]}")
         check_paged_status(self.device)
         return [done[i] for i in range(len(prompts))]

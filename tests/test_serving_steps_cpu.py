@@ -84,3 +84,22 @@ def test_a_step_that_raises_changes_nothing(monkeypatch, part, when):
     assert raised == 1
     assert [out[i] for i in range(len(PROMPTS))] == [greedy_text(p, 13) for p in PROMPTS]
     assert engine.cache.free_pages == 40
+
+
+@pytest.mark.parametrize("at", [0, 1, 5])
+def test_a_sequence_without_probabilities_leaves_alone(at):
+    """One sequence's logits become NaN after some tokens: it leaves with what it had and is named; the others' text is their own."""
+    bad = PROMPTS[1]
+    model = HistoryModel(spoil=lambda text: text[:len(bad)] == bad and len(text) >= len(bad) + at)
+    engine = PagedEngine(model, 40, 16, chunk=16, max_drafts=3, propose=_mostly_right)
+    for i, p in enumerate(PROMPTS):
+        engine.add(i, p, 13)
+    out = _run(engine)
+    assert list(engine.failed) == [1] and "no probabilities" in engine.failed[1]
+    assert out.pop(1, []) == greedy_text(bad, 13)[:at]
+    assert out == {i: greedy_text(p, 13) for i, p in enumerate(PROMPTS) if i != 1}
+    assert engine.cache.free_pages == 40
+    engine.add(1, [4], 2)
+    assert not engine.failed and _run(engine) == {1: greedy_text([4], 2)}
+    with pytest.raises(RuntimeError, match="no probabilities"):
+        PagedEngine(model, 40, 16).generate(PROMPTS, 13)
