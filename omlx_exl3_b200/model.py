@@ -385,10 +385,13 @@ class Qwen3EXL3(nn.Module):
     def forward_paged(self, tokens: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
                       rows: torch.Tensor | None = None) -> torch.Tensor:
         """The rows of several sequences at once (prompt chunks, decoded tokens, drafts): tokens (batch.total_rows) in the
-        batch's row order, appended to their pages. Returns this rank's logits of `rows` (all rows where None)."""
+        batch's row order, appended to their pages. Returns this rank's logits of `rows` (all rows where None, no head's product
+        where there are none)."""
         x = self.model.embed_tokens(tokens)
         for i, layer in enumerate(self.model.layers):
             x = layer.forward_paged(x, i, cache, batch, self.rope_cos, self.rope_sin)
+        if rows is not None and rows.numel() == 0:
+            return x.new_empty((0, x.shape[1] if self.lm_head is None else self.lm_head.out_features))
         h = self.model.norm(x if rows is None else x.index_select(0, rows))
         return self.lm_head(h) if self.lm_head is not None else h
 

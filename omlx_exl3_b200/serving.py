@@ -113,7 +113,7 @@ class PagedEngine:
             if wanted:
                 rows += range(at - len(drafts) - 1, at)
                 cu.append(len(rows))
-        logits = self.model.forward_paged(tokens, self.cache, batch, self._upload(rows, torch.int64) if rows else None)
+        logits = self.model.forward_paged(tokens, self.cache, batch, self._upload(rows, torch.int64))
         picked = self._verify(self.model.gather_logits(logits), judged, cu) if judged else []
         self._unchecked += 1
         if self.check_every and self._unchecked >= self.check_every:

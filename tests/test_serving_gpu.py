@@ -109,3 +109,17 @@ def test_engine_stops_samples_and_refuses(cuda):
     with pytest.raises(MemoryError):
         for _ in range(10):
             engine.step()
+
+
+def test_no_rows_wanted_means_no_head(cuda):
+    """A step of prompt chunks alone: the cache is filled, the vocabulary's projection is not run."""
+    model = _small_model(cuda, fuse=False, layers=1)
+    cache = model.make_paged_cache(16, 16)
+    cache.add(0)
+    ran = []
+    hook = model.lm_head.register_forward_hook(lambda *a: ran.append(1))
+    out = model.forward_paged(torch.arange(12, device=cuda), cache, cache.extend([(0, 12)]), torch.empty(0, dtype=torch.int64, device=cuda))
+    assert out.shape == (0, model.lm_head.out_features) and not ran and cache.k[0].any()
+    batch = cache.extend([(0, 1)])
+    assert model.forward_paged(torch.tensor([12], device=cuda), cache, batch).shape[0] == 1 and ran == [1]
+    hook.remove()

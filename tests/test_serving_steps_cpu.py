@@ -103,3 +103,11 @@ def test_a_sequence_without_probabilities_leaves_alone(at):
     assert not engine.failed and _run(engine) == {1: greedy_text([4], 2)}
     with pytest.raises(RuntimeError, match="no probabilities"):
         PagedEngine(model, 40, 16).generate(PROMPTS, 13)
+
+
+def test_steps_of_prompt_chunks_ask_for_no_logits():
+    """Only a prompt's last row and decoded rows need logits: a step without any asks for none."""
+    model = HistoryModel()
+    engine = PagedEngine(model, 40, 16, chunk=8, max_drafts=0)
+    assert engine.generate([PROMPTS[1]], 3) == [greedy_text(PROMPTS[1], 3)]
+    assert model.fed == [8] * 5 + [1, 1] and model.asked == [0] * 4 + [1, 1, 1]
