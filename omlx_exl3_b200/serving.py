@@ -12,6 +12,7 @@ accepted leaves the cache again, and the host reads one small tensor of tokens a
 """
 from __future__ import annotations
 
+import itertools
 from dataclasses import dataclass, field
 
 import torch
@@ -45,7 +46,8 @@ class _Sequence:
 class PagedEngine:
     def __init__(self, model: Qwen3EXL3, num_pages: int, page_size: int = 64, chunk: int = 512, max_drafts: int = 4,
                  propose=lookup_drafts, seed: int = 0, check_every: int = 64):
-        """chunk: prompt rows of a step; max_drafts: drafts of a sequence and step (0: none); propose(tokens, most) -> drafts."""
+        """chunk: prompt rows of a step; max_drafts: drafts of a sequence and step (0: none); propose(tokens, most) -> drafts, of
+        which no more than that are fed, and none from the first that is no token of the model on."""
         self.model, self.chunk, self.max_drafts, self.propose = model, chunk, max_drafts, propose
         self.device = model.rope_cos.device
         self.cache = model.make_paged_cache(num_pages, page_size)
@@ -66,9 +68,19 @@ class PagedEngine:
             raise ValueError("need a prompt, max_new of one or more and a temperature of zero or more")
         if len(prompt) + max_new > self.model.cfg.max_position_embeddings:
             raise ValueError(f"{len(prompt)} + {max_new} tokens exceed max_position_embeddings")
+        if not all(self._known(t) for t in prompt):                 # the embedding would fault on the GPU
+            raise ValueError("the prompt has tokens outside the model's vocabulary")
         self.cache.add(key)
         self.failed.pop(key, None)
         self._seqs[key] = _Sequence(list(prompt), len(prompt), max_new, float(temperature), frozenset(stop))
+
+    def _known(self, token: int) -> bool:
+        return 0 <= token < self.model.cfg.vocab_size
+
+    def _drafts(self, s: _Sequence) -> list[int]:
+        most = min(self.max_drafts, s.max_new - len(s.new) - 1)
+        drafts = list(self.propose(s.tokens, most))[:most] if most > 0 else []
+        return list(itertools.takewhile(self._known, drafts))
 
     def _upload(self, values: list, dtype) -> torch.Tensor:
         return torch.tensor(values, dtype=dtype).pin_memory().to(self.device, non_blocking=True)
@@ -87,8 +99,7 @@ class PagedEngine:
                 if n:
                     feeds.append((key, s, s.tokens[have:have + n], [], n == todo))
                 continue
-            left = s.max_new - len(s.new)
-            drafts = self.propose(s.tokens, min(self.max_drafts, left - 1))[:left - 1] if self.max_drafts and left > 1 else []
+            drafts = self._drafts(s)
             feeds.append((key, s, [s.tokens[-1]] + drafts, drafts, True))
         if not feeds:
             return {}

@@ -111,3 +111,25 @@ def test_steps_of_prompt_chunks_ask_for_no_logits():
     engine = PagedEngine(model, 40, 16, chunk=8, max_drafts=0)
     assert engine.generate([PROMPTS[1]], 3) == [greedy_text(PROMPTS[1], 3)]
     assert model.fed == [8] * 5 + [1, 1] and model.asked == [0] * 4 + [1, 1, 1]
+
+
+@pytest.mark.parametrize("propose", [
+    lambda t, n: [97] * n, lambda t, n: greedy_text(t, n)[:1] + [-1] * (n - 1), lambda t, n: [2 ** 40], lambda t, n: greedy_text(t, n + 6),
+    lambda t, n: tuple(greedy_text(t, n)),
+])
+def test_proposers_that_offer_too_much(propose):
+    """Drafts outside the vocabulary never reach the embedding, and no more than max_drafts are fed."""
+    model = HistoryModel()
+    engine = PagedEngine(model, 40, 16, max_drafts=2, propose=propose)
+    assert engine.generate([PROMPTS[0]], 9) == [greedy_text(PROMPTS[0], 9)]
+    assert max(model.fed[1:]) <= 3
+
+
+def test_add_refuses_tokens_that_the_model_does_not_have():
+    engine = PagedEngine(HistoryModel(), 40, 16)
+    for prompt in ([97], [1, -1, 2], [2 ** 40]):
+        with pytest.raises(ValueError, match="vocabulary"):
+            engine.add("x", prompt, 3)
+    assert engine.running == 0 and engine.step() == {}
+    engine.add("x", [96, 0], 3)
+    assert _run(engine) == {"x": greedy_text([96, 0], 3)}
