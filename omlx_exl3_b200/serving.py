@@ -48,6 +48,8 @@ class PagedEngine:
                  propose=lookup_drafts, seed: int = 0, check_every: int = 64):
         """chunk: prompt rows of a step; max_drafts: drafts of a sequence and step (0: none); propose(tokens, most) -> drafts, of
         which no more than that are fed, and none from the first that is no token of the model on."""
+        if chunk < 1 or max_drafts < 0:
+            raise ValueError("chunk must be one or more and max_drafts zero or more")
         self.model, self.chunk, self.max_drafts, self.propose = model, chunk, max_drafts, propose
         self.device = model.rope_cos.device
         self.cache = model.make_paged_cache(num_pages, page_size)
@@ -64,7 +66,7 @@ class PagedEngine:
 
     def add(self, key, prompt: list[int], max_new: int, temperature: float = 0.0, stop=()) -> None:
         """Queue a sequence; temperature 0 is greedy, `stop` are token ids that end it."""
-        if not prompt or max_new < 1 or temperature < 0:
+        if not prompt or max_new < 1 or not temperature >= 0:
             raise ValueError("need a prompt, max_new of one or more and a temperature of zero or more")
         if len(prompt) + max_new > self.model.cfg.max_position_embeddings:
             raise ValueError(f"{len(prompt)} + {max_new} tokens exceed max_position_embeddings")

@@ -130,6 +130,14 @@ def test_add_refuses_tokens_that_the_model_does_not_have():
     for prompt in ([97], [1, -1, 2], [2 ** 40]):
         with pytest.raises(ValueError, match="vocabulary"):
             engine.add("x", prompt, 3)
+    with pytest.raises(ValueError):
+        engine.add("x", [1], 3, temperature=float("nan"))
     assert engine.running == 0 and engine.step() == {}
     engine.add("x", [96, 0], 3)
     assert _run(engine) == {"x": greedy_text([96, 0], 3)}
+
+
+@pytest.mark.parametrize("kw", [dict(chunk=0), dict(chunk=-1), dict(max_drafts=-1)])
+def test_engine_refuses_sizes_that_it_cannot_step_with(kw):
+    with pytest.raises(ValueError):
+        PagedEngine(HistoryModel(), 40, 16, **kw)
