@@ -76,6 +76,10 @@ class PagedEngine:
         self.failed.pop(key, None)
         self._seqs[key] = _Sequence(list(prompt), len(prompt), max_new, float(temperature), frozenset(stop))
 
+    def _drop(self, key) -> None:
+        self.cache.release(key)
+        del self._seqs[key]
+
     def _known(self, token: int) -> bool:
         return 0 <= token < self.model.cfg.vocab_size
 
@@ -164,22 +168,27 @@ class PagedEngine:
             if dead and not ended:
                 self.failed[key] = "the model gave no probabilities"
             if dead or ended:
-                self.cache.release(key)
-                del self._seqs[key]
+                self._drop(key)
             elif lengths[key] >= s.prompt:                          # its last token and the drafts that stand stay cached
                 self.cache.truncate(key, lengths[key] + len(got))
         return out
 
     def generate(self, prompts: list[list[int]], max_new: int, temperature: float = 0.0, stop=()) -> list[list[int]]:
-        """All of the prompts' continuations."""
+        """All of the prompts' continuations, by an engine that runs nothing else. If it raises, none of them stays behind."""
+        if self._seqs:
+            raise ValueError("generate needs an engine without running sequences")
         done = {i: [] for i in range(len(prompts))}
-        for i, p in enumerate(prompts):
-            self.add(i, p, max_new, temperature, stop)
-        while self.running:
-            for i, got in self.step().items():
-                done[i] += got
-            for i in done:
-                if i in self.failed:
-                    raise RuntimeError(f"prompt {i}: {self.failed[i]}")
-        check_paged_status(self.device)
+        try:
+            for i, p in enumerate(prompts):
+                self.add(i, p, max_new, temperature, stop)
+            while self.running:
+                for i, got in self.step().items():
+                    done[i] += got
+                for i in done:
+                    if i in self.failed:
+                        raise RuntimeError(f"prompt {i}: {self.failed[i]}")
+            check_paged_status(self.device)
+        finally:
+            for key in list(self._seqs):
+                self._drop(key)
         return [done[i] for i in range(len(prompts))]

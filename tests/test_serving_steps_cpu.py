@@ -141,3 +141,29 @@ def test_add_refuses_tokens_that_the_model_does_not_have():
 def test_engine_refuses_sizes_that_it_cannot_step_with(kw):
     with pytest.raises(ValueError):
         PagedEngine(HistoryModel(), 40, 16, **kw)
+
+
+def test_generate_beside_other_sequences_is_refused():
+    """It would take the others' tokens and lose them."""
+    engine = PagedEngine(HistoryModel(), 40, 16)
+    engine.add("mine", PROMPTS[0], 6)
+    with pytest.raises(ValueError, match="running"):
+        engine.generate([PROMPTS[2]], 4)
+    assert _run(engine) == {"mine": greedy_text(PROMPTS[0], 6)}
+    assert engine.generate([PROMPTS[2]], 4) == [greedy_text(PROMPTS[2], 4)]
+
+
+def test_generate_that_raises_leaves_nothing_behind():
+    """A prompt that is refused, a step that fails: the engine is empty again and the next call is a fresh one."""
+    def fail(step):
+        if step == 2:
+            raise Broken
+    model = HistoryModel(fail)
+    engine = PagedEngine(model, 40, 16)
+    with pytest.raises(ValueError):
+        engine.generate([PROMPTS[0], []], 5)
+    assert engine.running == 0 and engine.cache.free_pages == 40
+    with pytest.raises(Broken):
+        engine.generate(PROMPTS, 5)
+    assert engine.running == 0 and engine.cache.free_pages == 40
+    assert engine.generate(PROMPTS, 5) == [greedy_text(p, 5) for p in PROMPTS]
