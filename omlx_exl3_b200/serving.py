@@ -57,6 +57,7 @@ class PagedEngine:
         self._gen = torch.Generator(device=self.device)
         self._gen.manual_seed(seed)
         self._seqs: dict = {}
+        self._set_back: set = set()                                 # sequences that gave their pages up and wait
         self.failed: dict = {}                                      # sequences that left without an end, and why
         self.drafted = self.accepted = 0
 
@@ -79,6 +80,13 @@ class PagedEngine:
     def _drop(self, key) -> None:
         self.cache.release(key)
         del self._seqs[key]
+        self._set_back.clear()                                      # pages came back: all may try again
+
+    def cancel(self, key) -> None:
+        """A sequence leaves the engine, whatever it was doing; its pages come back. KeyError if there is none under `key`."""
+        if key not in self._seqs:
+            raise KeyError(key)
+        self._drop(key)
 
     def _known(self, token: int) -> bool:
         return 0 <= token < self.model.cfg.vocab_size
@@ -94,21 +102,25 @@ class PagedEngine:
     def step(self) -> dict:
         """One batch; returns the new tokens of the sequences that have some (finished ones leave the engine). A step that raises
         changes nothing: the next one feeds the same rows. A sequence for which the model gives no probabilities leaves too, and
-        `failed` names it."""
-        feeds, room = [], self.chunk
-        for key, s in self._seqs.items():
-            have = self.cache.length(key)
-            todo = s.prompt - have
-            if todo > 0:                                            # its prompt, as far as this step's chunk goes
-                n = min(todo, room)
-                room -= n
-                if n:
-                    feeds.append((key, s, s.tokens[have:have + n], [], n == todo))
-                continue
-            drafts = self._drafts(s)
-            feeds.append((key, s, [s.tokens[-1]] + drafts, drafts, True))
-        if not feeds:
+        `failed` names it.
+
+        Where the pool is short of pages, drafts are left out first, then prompts wait; if nothing can be fed, the youngest sequence
+        gives its pages up and is read again once another has left. MemoryError, naming them, if all that is left are sequences
+        that the whole pool could not hold (cancel() them)."""
+        if not self._seqs:
             return {}
+        feeds = self._feeds()
+        while not feeds:
+            holders = [key for key in self._seqs if self.cache.length(key)]
+            if len(holders) > 1:
+                self._give_up(holders[-1])
+                self._set_back.add(holders[-1])
+            elif self._set_back:
+                self._set_back.clear()
+            else:
+                keys = ", ".join(repr(key) for key in self._seqs)
+                raise MemoryError(f"the pool of {self.cache.num_pages} pages cannot hold the next token of {keys}")
+            feeds = self._feeds()
         judged = [(key, s, drafts) for key, s, _, drafts, wanted in feeds if wanted]
         lengths = {key: self.cache.length(key) for key, *_ in feeds}
         try:
@@ -118,6 +130,53 @@ class PagedEngine:
                 self.cache.truncate(key, length)
             raise
         return self._keep(judged, picked, lengths)
+
+    def _give_up(self, key) -> None:
+        """A sequence's pages come back; all it has is its prompt from now on."""
+        self.cache.truncate(key, 0)
+        self._seqs[key].prompt = len(self._seqs[key].tokens)
+
+    def _feeds(self) -> list:
+        """What the next step feeds, as (key, sequence, rows, drafts, whether logits are wanted), within the free pages: a row of
+        every decoding sequence, prompts in order of arrival, then drafts."""
+        size = self.cache.page_size
+        reading, decoding, drafts = [], [], {}
+        for key, s in self._seqs.items():
+            if len(s.tokens) > self.cache.num_pages * size:         # the whole pool could not hold what its next token needs
+                if self.cache.length(key):
+                    self._give_up(key)
+            elif self.cache.length(key) < s.prompt:
+                reading.append(key)
+            else:
+                decoding.append(key)
+        spare, grant = self.cache.free_pages, {}
+
+        def take(key, want):                                        # rows granted, of the `want` more that the sequence would have
+            nonlocal spare
+            at = self.cache.length(key) + grant.get(key, 0)
+            held = -(-at // size)
+            n = max(0, min(want, (held + spare) * size - at))
+            spare -= -(-(at + n) // size) - held
+            if n:
+                grant[key] = grant.get(key, 0) + n
+            return n
+
+        decoding = [key for key in decoding if take(key, 1)]
+        room = self.chunk
+        for key in reading:
+            if room and key not in self._set_back:
+                room -= take(key, min(self._seqs[key].prompt - self.cache.length(key), room))
+        for key in decoding:
+            offered = self._drafts(self._seqs[key])
+            drafts[key] = offered[:take(key, len(offered))]
+        feeds = []
+        for key, s in self._seqs.items():
+            if key in drafts:
+                feeds.append((key, s, [s.tokens[-1]] + drafts[key], drafts[key], True))
+            elif key in grant:                                      # its prompt, as far as this step's chunk goes
+                have = self.cache.length(key)
+                feeds.append((key, s, s.tokens[have:have + grant[key]], [], have + grant[key] == s.prompt))
+        return feeds
 
     def _run(self, feeds: list, judged: list) -> list:
         """The batch through the model and the verification; for each judged sequence its tokens and their count."""

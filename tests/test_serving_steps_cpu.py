@@ -167,3 +167,51 @@ def test_generate_that_raises_leaves_nothing_behind():
         engine.generate(PROMPTS, 5)
     assert engine.running == 0 and engine.cache.free_pages == 40
     assert engine.generate(PROMPTS, 5) == [greedy_text(p, 5) for p in PROMPTS]
+
+
+@pytest.mark.parametrize("pages", [6, 7, 8, 9, 12, 20])
+@pytest.mark.parametrize("chunk,drafts", [(512, 3), (5, 0), (16, 3)])
+def test_a_nearly_full_pool_finishes_everything(pages, chunk, drafts):
+    """16 positions a page: each sequence alone needs up to 6 pages, all together 20. Whatever is short waits, or is read again."""
+    prompts = [list(range(10 + i, 10 + i + n)) for i, n in enumerate((40, 3, 58, 20, 1))]
+    engine = PagedEngine(HistoryModel(), pages, 16, chunk=chunk, max_drafts=drafts, propose=_mostly_right)
+    for i, p in enumerate(prompts):
+        engine.add(i, p, 35)
+    assert _run(engine) == {i: greedy_text(p, 35) for i, p in enumerate(prompts)}
+    assert engine.cache.free_pages == pages
+
+
+def test_what_the_pool_can_never_hold_does_not_stop_the_others():
+    """A prompt longer than the pool, and a sequence that outgrows it: the others finish, then MemoryError names them; cancelled,
+    they are gone."""
+    engine = PagedEngine(HistoryModel(), 6, 16, chunk=16, max_drafts=0)
+    engine.add("long", [7] * 97, 2)
+    engine.add("grows", [8] * 60, 60)
+    for i, p in enumerate(PROMPTS):
+        engine.add(i, p, 13)
+    out = {}
+    with pytest.raises(MemoryError, match="'long', 'grows'"):
+        _run(engine, out)
+    assert out.pop("grows") == greedy_text([8] * 60, 37)               # its 97th token needs a position for its 98th
+    assert out == {i: greedy_text(p, 13) for i, p in enumerate(PROMPTS)}
+    with pytest.raises(MemoryError):
+        engine.step()
+    engine.cancel("long")
+    engine.cancel("grows")
+    assert engine.running == 0 and engine.cache.free_pages == 6 and engine.step() == {}
+    with pytest.raises(KeyError):
+        engine.cancel("long")
+
+
+def test_cancel_in_the_middle():
+    engine = PagedEngine(HistoryModel(), 40, 16, chunk=16, max_drafts=2, propose=_mostly_right)
+    for i, p in enumerate(PROMPTS):
+        engine.add(i, p, 13)
+    out = {}
+    for _ in range(3):
+        for key, tokens in engine.step().items():
+            out.setdefault(key, []).extend(tokens)
+    engine.cancel(1)
+    out.pop(1, None)
+    assert _run(engine, out) == {i: greedy_text(p, 13) for i, p in enumerate(PROMPTS) if i != 1}
+    assert engine.cache.free_pages == 40
