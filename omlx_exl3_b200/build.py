@@ -56,7 +56,7 @@ def up_to_date() -> bool:
 
 def binding_up_to_date() -> bool:
     return BINDING.exists() and all(p.stat().st_mtime <= BINDING.stat().st_mtime
-                                    for p in [BINDING_SRC, *INCLUDE.glob("*.h")])
+                                    for p in [BINDING_SRC, Path(__file__), *INCLUDE.glob("*.h")])
 
 
 def build_binding(force: bool = False) -> Path:
@@ -72,7 +72,10 @@ def build_binding(force: bool = False) -> Path:
            "-isystem", str(troot / "include"), "-isystem", str(troot / "include" / "torch" / "csrc" / "api" / "include"),
            "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_path("include"), f"-I{INCLUDE}",
            str(BINDING_SRC), "-o", str(tmp), f"-L{PKG}", "-lexl3b200", f"-L{troot / 'lib'}", "-ltorch_python", "-ltorch",
-           "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+           "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN",
+           # the C++ runtime that torch has loaded, whatever the compiler would link: with a second one inside the binding (a
+           # toolchain that has only libstdc++.a) a message that formats a number ends the process
+           "-nostdlib++", "-l:libstdc++.so.6"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed on {BINDING_SRC.name}:\n{r.stdout}\n{r.stderr}")
