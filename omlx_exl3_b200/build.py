@@ -54,13 +54,19 @@ def up_to_date() -> bool:
     return all(p.stat().st_mtime <= t for p in _deps())
 
 
+def _binding_target() -> str:
+    """The torch and interpreter a binding is compiled against, as it carries them in its docstring."""
+    import torch
+    return f"built for torch {torch.__version__}, {sys.implementation.cache_tag}"
+
+
 def binding_up_to_date() -> bool:
-    return BINDING.exists() and all(p.stat().st_mtime <= BINDING.stat().st_mtime
-                                    for p in [BINDING_SRC, Path(__file__), *INCLUDE.glob("*.h")])
+    return (BINDING.exists() and all(p.stat().st_mtime <= BINDING.stat().st_mtime for p in [BINDING_SRC, Path(__file__), *INCLUDE.glob("*.h")])
+            and f"{_binding_target()}\0".encode() in BINDING.read_bytes())
 
 
 def build_binding(force: bool = False) -> Path:
-    """Compile the torch binding (when its source changed); the library has to be there."""
+    """Compile the torch binding (when its source or the installed torch changed); the library has to be there."""
     if not force and binding_up_to_date():
         return BINDING
     import torch
@@ -68,7 +74,7 @@ def build_binding(force: bool = False) -> Path:
     cuda = Path(nvcc()).resolve().parent.parent if shutil.which(nvcc()) else Path("/usr/local/cuda")
     tmp = BINDING.with_suffix(f".so.{os.getpid()}.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DEXL3_BUILT_FOR="{_binding_target()}"',
            "-isystem", str(troot / "include"), "-isystem", str(troot / "include" / "torch" / "csrc" / "api" / "include"),
            "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_path("include"), f"-I{INCLUDE}",
            str(BINDING_SRC), "-o", str(tmp), f"-L{PKG}", "-lexl3b200", f"-L{troot / 'lib'}", "-ltorch_python", "-ltorch",

@@ -328,7 +328,7 @@ PyObject* status(PyObject*, PyObject* const* arg, Py_ssize_t n)
 #define CALL(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {CALL(paged_qkv_post), CALL(paged_attn), CALL(verify_drafts), CALL(status), CALL(take_status),
                          {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_exl3_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_exl3_torch", EXL3_BUILT_FOR, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 

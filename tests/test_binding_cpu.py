@@ -1,5 +1,21 @@
-"""CPU: how the torch binding is built: on the C++ runtime that torch has loaded."""
+"""CPU: how the torch binding is built: for one torch and interpreter, on the C++ runtime that they have loaded."""
+import sys
+
 import pytest
+import torch
+
+
+def test_another_torch_means_another_build(monkeypatch):
+    from omlx_exl3_b200 import _lib, build
+    assert _lib.torch_calls().__doc__ == f"built for torch {torch.__version__}, {sys.implementation.cache_tag}"
+    assert build.binding_up_to_date()
+    with monkeypatch.context() as m:
+        m.setattr(torch, "__version__", torch.__version__ + "0")
+        assert not build.binding_up_to_date()
+    with monkeypatch.context() as m:
+        m.setattr(torch, "__version__", "1.0")
+        assert not build.binding_up_to_date()
+    assert build.binding_up_to_date()
 
 
 @pytest.mark.parametrize("compiler", [None, "g++"])
