@@ -135,9 +135,10 @@ __global__ void __launch_bounds__(kPmThreads) paged_merge_kernel(const __grid_co
     const bool is_few = block < few_blocks;
     const PaArgs& a = is_few ? few : tiles;
     const PaItem g = a.items[blockIdx.x];
+    const int first_row = a.b.cu_rows[0], end_row = a.b.cu_rows[a.b.seqs];
     {                                                 // rows before the first sequence's and behind the last one's: zeros
         const size_t row16 = (size_t)a.hq * HD / 8, n = row16 * a.b.rows, threads = (size_t)gridDim.x * gridDim.y * kPmThreads;
-        const size_t lead = g.parts < 0 ? n : row16 * a.b.cu_rows[0], gap = g.parts < 0 ? 0 : row16 * a.b.cu_rows[a.b.seqs] - lead;
+        const size_t lead = g.parts < 0 ? n : row16 * first_row, gap = g.parts < 0 ? 0 : row16 * end_row - lead;
         for (size_t i = (blockIdx.y * gridDim.x + blockIdx.x) * kPmThreads + threadIdx.x; i + gap < n; i += threads)
             reinterpret_cast<uint4*>(a.out)[i < lead ? i : i + gap] = make_uint4(0, 0, 0, 0);
     }

@@ -94,10 +94,13 @@ __global__ void __launch_bounds__(128, 6) paged_post_kernel(const PagedPostArgs 
     for (int u = 0; u < U; ++u) fetch(u, part * PER + u * stride);
     const int s = seq_of_row(b.cu_rows, b.seqs, row, lane);
     const int start = b.cu_rows[s], end = b.cu_rows[s + 1], pos = b.lens[s] - end + row;
-    const bool astray = (row < start && s > 0) || (row >= end && s + 1 < b.seqs);      // cu_rows does not rise here
-    const bool pad = pos < 0 || row >= end || row < start, known = pos < a.rope_rows;
+    const bool inside = row >= start && row < end, pad = pos < 0 || !inside, known = pos < a.rope_rows;
     const int page = page_of(b, s, pos);
-    if ((astray || (!pad && (!known || page < 0))) && lane == 0 && part == 0) atomicOr(a.status, kStatusPagedRange);
+    if ((pad || !known || page < 0) && lane == 0 && part == 0) {
+        // a row that its sequence does not have, though it is neither the first's nor the last's: cu_rows falls there
+        const bool astray = (row < start && s > 0) || (row >= end && s + 1 < b.seqs);
+        if (astray || !pad) atomicOr(a.status, kStatusPagedRange);
+    }
     const bool append = !pad && known && page >= 0, has_q = !pad && known;
     float co[4] = {}, si[4] = {};
     if (rotated && has_q) {

@@ -80,20 +80,22 @@ struct PaSched {
     }
     __device__ __forceinline__ static int units_of(int end) { return max(1, (end + kPaStep - 1) / kPaStep); }
 
-    // Rows and length of sequence q: a length that could not be one is taken as the nearest that could.
-    __device__ __forceinline__ void load(int q, int& r, int& n) const
+    // Rows and length of sequence q: a length that could not be one is taken as the nearest that could. False where the rows are out
+    // of order or of range; all three words are asked for before any is looked at.
+    __device__ __forceinline__ bool load(int q, int& r, int& n) const
     {
-        r = a.b.cu_rows[q + 1] - a.b.cu_rows[q];      // start() has seen that this lies in 0 .. b.rows
-        n = max(0, min(a.b.lens[q], cap + a.b.rows));
+        const int lo = a.b.cu_rows[q], hi = a.b.cu_rows[q + 1], len = a.b.lens[q];
+        r = hi - lo;
+        n = max(0, min(len, cap + a.b.rows));
+        return (lo >= 0) & (hi >= lo) & (hi <= a.b.rows);
     }
 
     // Length of sequence q in the list, for one kv head; -1: its rows are out of order or out of range.
     __device__ __forceinline__ int head_length(int q) const
     {
         if (q >= a.b.seqs) return 0;
-        if (a.b.cu_rows[q] < 0 || a.b.cu_rows[q + 1] < a.b.cu_rows[q] || a.b.cu_rows[q + 1] > a.b.rows) return -1;
         int r, n, sum = 0;
-        load(q, r, n);
+        if (!load(q, r, n)) return -1;
         if (!takes(r)) return 0;
         for (int i = 0; i * a.span < r * a.grp; ++i) sum += units_of(item_end(r, n, i)) + a.item;
         return sum;
