@@ -19,8 +19,9 @@
 // the sum is fp32 of the unrounded p), by the softmax thread itself, once the P V issued last is complete.
 //
 // Bound by the softmax (ex2: 128 x 128 of a tile step take 1024 cycles of the special function unit, as long as its 2 x 128^3
-// MMAs) and by what lies between: 1.06 PFLOP/s, 0.65 of a measured library GEMM, for 4096 rows over 8192 positions of
-// 40 / 8 heads of 128 in bf16 (486 us); an exponent polynomial on the FMA pipe for a quarter of the ex2 (553 against 507
+// MMAs) and by what lies between (both are busy 54 % of the time): 4096 rows over 8192 positions of 40 / 8 heads of 128 in bf16 take
+// 486 us in short runs, 1.06 PFLOP/s, 0.65 of a measured library GEMM's burst, and 556 us in a long loop, where the power cap lowers
+// the clocks: 0.93 PFLOP/s, 0.68 of its sustained rate; an exponent polynomial on the FMA pipe for a quarter of the ex2 (553 against 507
 // us at that stage), four softmax warpgroups with a row's halves in two threads (589), and whole steps with an enforced
 // alternation of the slots' MMAs (497) were measured slower.
 //
@@ -758,13 +759,15 @@ extern "C" int exl3_paged_attn(const exl3_paged_desc* batch, const void* q, long
     // start, which counts while the SMs outnumber the pairs of a sequence and a kv head; 16 rows at a time read the keys and
     // values once per 16. Measured, us with sequences of up to 32 / up to 64 packed rows on the latter, each of 1 to 8 rows in
     // groups of 5 heads: 9 over 1000 positions of 8 kv heads 22.0 / 18.9, 16 26.8 / 21.9, 16 over 8000 41.4 / 44.3, 32 57.4 / 65.5, 64
-    // 98.2 / 122.3, 128 127.4 / 142.4; of 4 kv heads 9 over 8000 26.8 / 23.0, 32 39.6 / 38.9, 64 61.6 / 71.6. (Up to 16: 64 over
+    // 98.2 / 122.3, 128 127.4 / 142.4; of 4 kv heads 9 over 8000 26.8 / 23.0, 32 39.6 / 38.9, 64 61.6 / 71.6. So the limit is 64 where
+    // the pairs of sequence and kv head are no more than the SMs. What also counts is the length, which the host does not know: at 128
+    // pairs the rule takes the faster side over 1000 positions (by 5 us) and the slower one over 8000 (by 3). (Up to 16: 64 over
     // 8000 95.5, but 1 to 5 rows 42.7 / 39.4 at 16 / 32.) A batch with a row per sequence at most is taken for single tokens:
     // one launch, right whatever the rows are. Where both run, the kernel for few rows comes second and waits for the tiles at
-    // its end only: 13 sequences of 1 to 777 rows 54.6 us, and 58.7 one after the other.
+    // its end only: 13 sequences of 1 to 777 rows 54.8 us, and 58.7 one after the other.
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const long long packed = (long long)batch->rows * a.grp;
-        const int hi = packed <= 32ll * batch->seqs && (long long)batch->seqs * batch->hkv <= attn_ctas() ? 64 : 32;
+    const int hi = packed <= 32ll * batch->seqs && (long long)batch->seqs * batch->hkv <= attn_ctas() ? 64 : 32;
     const long long most = max_rows > 0 && max_rows < batch->rows ? (long long)max_rows * a.grp : packed;
     const bool few_only = most <= hi || (batch->rows <= batch->seqs && a.grp <= hi);
     const bool tiles_only = !few_only && (batch->seqs == 1 || a.grp > hi);

@@ -10,9 +10,9 @@
 // by 2^8 (no cross-lane reduction on the usual path), P^T turned from accumulator to operand by movmatrix, and
 // O^T += V^T P^T. At an item's end the warps' (m, l, O) are merged through shared memory in warp order.
 //
-// Bound by the cache's bytes where there are many: two sequences at 65,000 positions, 533 MB in 86 us (6.2 TB/s, 0.95 of a
-// measured copy); 64 of 1 to 8192, 385 MB in 70 us (5.5 TB/s); by launch and the chain of dependent loads (lengths, page,
-// keys) for one short one (9.2 us at 4097 positions).
+// Bound by the cache's bytes where there are many: two sequences at 65,000 positions, 533 MB in 87 us (6.1 TB/s, 0.93 of a
+// measured copy); 64 of 1 to 8192, 385 MB in 69 us (5.5 TB/s, 0.85); by launch and the chain of dependent loads (lengths, page,
+// keys) for one short one (9.4 us at 4097 positions).
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -3,8 +3,9 @@
 //
 //   xn = x * rsqrt(mean(x^2) + eps) * w ;  (a, b) = (xn[c], xn[c + R]) -> (a cos - b sin, b cos + a sin), c < R
 //
-// Bound by the rows' bytes where there are many (3428 rows of 40 + 2 x 8 heads of 128, 100 MB in 23.7 us, 4.2 TB/s, 0.65 of a
-// measured copy, which so short a pass does not reach), by launch and dependent loads where there are few (2.9 us).
+// Where there are many rows, bound by issue (64 % of the slots; DRAM is a quarter busy) and the rounds of loads of one wave: 3428
+// rows of 40 + 2 x 8 heads of 128, 100 MB in 23.7 us, 4.2 TB/s, 0.65 of a measured copy. Where there are few, by launch and
+// dependent loads (2.8 us).
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -9,6 +9,8 @@ accepted leaves the cache again, and the host reads one small tensor of tokens a
     engine.add("a", prompt_ids, max_new=200, temperature=0.7)
     while engine.running:
         for key, tokens in engine.step().items(): ...
+
+cancel() drops a sequence; engine.failed names those that left because the model gave no probabilities for them.
 """
 from __future__ import annotations
 
