@@ -358,16 +358,14 @@ __global__ void __launch_bounds__(32 * kDecideWarps) verify_decide_kernel(const 
         const int banned = at.token >= 0 && at.token < a.n ? (int)at.token : -1;
         // Columns of this thread in rising order; MODE 0: w = p, 1: w = p - q, 2: w = p but for the rejected token (one-hot q).
         // Threads, warps and CTAs all compare the rounded quotients w / noise, so the answer is the first column of the largest
-        // however the columns are shared out. A thread asks for w >= low * noise first, low a little under its best: a larger
-        // quotient always passes (the two products' roundings are within 2^-22), and the division is for the few that do.
+        // however the columns are shared out. A thread asks for w >= best * noise first: a quotient that rounds to more than best is
+        // more than best, so w is at least the product, rounded too; the division is for the few columns that pass.
         auto race = [&](auto mode, float& best, int& idx) {
             constexpr int MODE = decltype(mode)::value;
-            float low = best;
             auto take = [&](int v, float w, float nz) {
                 const float r = w / nz;
                 if (r > best) {
                     best = r;
-                    low = r * (1.f - 0x1p-22f);
                     idx = v;
                 }
             };
@@ -392,18 +390,18 @@ __global__ void __launch_bounds__(32 * kDecideWarps) verify_decide_kernel(const 
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     w[i] = weight(v + i, to_f32(xe[i]), to_f32(de[i]));
-                    any |= w[i] >= low * nz[i];
+                    any |= w[i] >= best * nz[i];
                 }
                 if (any) {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i)
-                        if (w[i] >= low * nz[i]) take(v + i, w[i], nz[i]);
+                        if (w[i] >= best * nz[i]) take(v + i, w[i], nz[i]);
                 }
             }
 #pragma unroll 4
             for (int v = whole + me; v < a.n; v += threads) {
                 const float w = weight(v, to_f32(tr[v]), MODE == 1 ? to_f32(dr[v]) : 0.f), nz = e[v];
-                if (w >= low * nz) take(v, w, nz);
+                if (w >= best * nz) take(v, w, nz);
             }
         };
         // first the residual, then (where that is zero everywhere) p itself
